@@ -355,6 +355,95 @@ int jq_sample_softmax(const jq_batch *b, const int32_t *d_counts, const int32_t 
                       int32_t cap, uint64_t seed, uint64_t ply, int32_t *d_compact_actions,
                       int32_t *d_world_actions, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Policy operators: what stands between a network's features and the action
+ * that jq_ply takes, and its training.  They need no jq_init and no batch;
+ * no counterpart in the reference, whose networks are torch modules.  Arrays
+ * are device pointers, rows are `*_stride` elements apart with neighbouring
+ * places next to each other (a stride of 0 repeats one row); outputs are
+ * contiguous.  Aligned to their elements is enough; rows that all start on
+ * 16 bytes take the widest loads.  Equal calls give equal bits.
+ * ------------------------------------------------------------------------- */
+
+/* Element types of features, logits and weights. */
+enum { JQ_F32 = 0, JQ_F16 = 1, JQ_BF16 = 2 };
+
+#define JQ_POLICY_MAX_ACTIONS (1 << 18) /* places of one row of logits */
+#define JQ_POLICY_MAX_DRAFTS 1024       /* drafted actions of one game */
+
+/* Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight +
+ * bias (either may be NULL: 1 and 0).  x, y are `dtype`, weight and bias
+ * `wdtype` (JQ_F32 or `dtype`); statistics are 32-bit.  d_stats (rows x 3
+ * floats: mean, what its rounding left, 1 / sqrt(var + eps)) is what the
+ * backward pass reads, NULL when there will be none.  rows >= 1, dim >= 1. */
+int jq_layer_norm(const void *d_x, int64_t x_stride, const void *d_weight, const void *d_bias, int64_t rows,
+                  int32_t dim, int32_t dtype, int32_t wdtype, float eps, void *d_y, float *d_stats, void *stream);
+
+/* Gradients of jq_layer_norm from dy (`dtype`): d_dx (`dtype`), d_dweight and
+ * d_dbias (`wdtype`, summed over the rows in a fixed order); each may be
+ * NULL.  d_scratch: jq_layer_norm_scratch_floats(rows, dim) floats, needed
+ * for d_dweight and d_dbias, used by one call at a time. */
+int64_t jq_layer_norm_scratch_floats(int64_t rows, int32_t dim);
+int jq_layer_norm_backward(const void *d_x, int64_t x_stride, const void *d_weight, const void *d_dy,
+                           int64_t dy_stride, const float *d_stats, int64_t rows, int32_t dim, int32_t dtype,
+                           int32_t wdtype, void *d_dx, void *d_dweight, void *d_dbias, float *d_scratch,
+                           void *stream);
+
+/* log-probability of d_actions[row] and entropy of the row's softmax over its
+ * legal places (d_mask nonzero; NULL: all), both float32.  Masked logits are
+ * not looked at.  An action outside [0, actions) is "no action": 0.  One
+ * that is not legal, or whose logit is -inf: -inf.  A row without a legal
+ * place above -inf has entropy 0.  NaN or +inf at a legal place: NaN.
+ * For the backward pass: d_stats (rows x 4 floats, 16-byte aligned) and, with
+ * a mask, d_bits (rows x ceil(actions / 32) words), the mask in bits; both
+ * NULL when there will be none. */
+int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, const uint8_t *d_mask,
+                       int64_t mask_stride, const int32_t *d_actions, int64_t rows, int32_t actions,
+                       float *d_log_prob, float *d_entropy, float *d_stats, uint32_t *d_bits, void *stream);
+
+/* Gradient of the logits (`dtype`, every place: 0 where masked) from those of
+ * the log-probabilities and entropies (float32, `*_stride` floats apart;
+ * NULL: 0).  d_bits NULL: there was no mask.  A log-probability that does not
+ * depend on the logits (no action, or -inf) has no gradient. */
+int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_t dtype, const uint32_t *d_bits,
+                                const int32_t *d_actions, const float *d_stats, const float *d_grad_log_prob,
+                                int64_t grad_log_prob_stride, const float *d_grad_entropy,
+                                int64_t grad_entropy_stride, int64_t rows, int32_t actions, void *d_dlogits,
+                                void *stream);
+
+/* Verification of drafted actions against a target policy, from given random
+ * numbers in [0, 1).  Per game, with p_i the target's probabilities at place
+ * i and q_i the draft's (d_draft_logits NULL: certain of the drafted action),
+ * both over the place's legal set: drafted action a_i is kept while
+ * accept_u_i q_i(a_i) < p_i(a_i).  At the first one that is not, the action
+ * is drawn from max(p_i - q_i, 0) (from p_i where that leaves less than
+ * 2^-40); after the last, from p at the place behind it.  Drawing takes the
+ * least action whose running sum exceeds sample_u times the total.  What
+ * comes out is distributed as the target's own play.  Computed in 64 bits.
+ *
+ * Outputs per game: `accepted` kept drafts; out_actions (drafts + 1): the
+ * kept drafts, the drawn action, then -1; log_probs (drafts + 1): the
+ * target's log-probability of each, 0 behind them.  A place without legal
+ * actions draws -1 with log-probability 0; one with NaN or +inf at a legal
+ * place, -1 with NaN.  Drafted actions outside [0, actions) or not legal are
+ * not kept.  With drafts = 0 this samples one action per game. */
+typedef struct jq_drafts {
+    int32_t games, drafts, actions, dtype;
+    const void *logits;               /* (games, drafts + 1, actions) */
+    int64_t logits_game, logits_place;
+    const void *draft_logits;         /* (games, drafts, actions), `dtype`; or NULL */
+    int64_t draft_game, draft_place;
+    const uint8_t *mask;              /* (games, drafts + 1, actions); NULL: all legal */
+    int64_t mask_game, mask_place;
+    const int32_t *drafted;           /* (games, drafts) */
+    const int32_t *lengths;           /* (games) drafts in use, cut to [0, drafts]; NULL: all */
+    const float *accept_u, *sample_u; /* (games, drafts), (games) */
+    int32_t *accepted, *out_actions;  /* (games), (games, drafts + 1) */
+    float *log_probs;                 /* (games, drafts + 1) */
+} jq_drafts;
+
+int jq_verify_drafts(const jq_drafts *d, void *stream);
+
 /* Per-CTA timestamps of the last obs_kernel (kernel 0) or rules_kernel
  * (kernel 1) launch: `ctas` rows of 8 uint64 (globaltimer ns at fixed points
  * of the kernel; see junqi_b200/csrc/jq_trace.cuh), copied to host memory.

@@ -56,10 +56,24 @@ class JqStepOut(ctypes.Structure):
                  "zobrist")]
 
 
+F32, F16, BF16 = 0, 1, 2  # element types of the policy operators
+POLICY_MAX_ACTIONS, POLICY_MAX_DRAFTS = 1 << 18, 1024
+
+
+class JqDrafts(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("games", "drafts", "actions", "dtype")] + \
+        [("logits", ctypes.c_void_p), ("logits_game", ctypes.c_int64), ("logits_place", ctypes.c_int64),
+         ("draft_logits", ctypes.c_void_p), ("draft_game", ctypes.c_int64), ("draft_place", ctypes.c_int64),
+         ("mask", ctypes.c_void_p), ("mask_game", ctypes.c_int64), ("mask_place", ctypes.c_int64)] + \
+        [(n, ctypes.c_void_p) for n in ("drafted", "lengths", "accept_u", "sample_u", "accepted", "out_actions",
+                                        "log_probs")]
+
+
 # exported name -> (restype, argtypes)
 _vp, _i32, _i64, _u64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
 _PB = ctypes.POINTER(JqBatch)
 _PO = ctypes.POINTER(JqStepOut)
+_f32 = ctypes.c_float
 SIGNATURES = {
     "jq_abi_version": (ctypes.c_int, []),
     "jq_last_error": (ctypes.c_char_p, []),
@@ -92,6 +106,14 @@ SIGNATURES = {
     "jq_cell_beliefs_update": (ctypes.c_int, [_PB, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "jq_sample_uniform": (ctypes.c_int, [_i32, _vp, _vp, _i32, _u64, _u64, _vp, _vp]),
     "jq_sample_softmax": (ctypes.c_int, [_PB, _vp, _vp, _i32, _u64, _u64, _vp, _vp, _vp]),
+    "jq_layer_norm": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _vp]),
+    "jq_layer_norm_scratch_floats": (_i64, [_i64, _i32]),
+    "jq_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp,
+                                              _vp, _vp]),
+    "jq_action_log_prob": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "jq_action_log_prob_backward": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i32,
+                                                   _vp, _vp]),
+    "jq_verify_drafts": (ctypes.c_int, [ctypes.POINTER(JqDrafts), _vp]),
     "jq_trace_read": (ctypes.c_int, [_i32, _vp, _i32]),
 }
 

@@ -18,7 +18,9 @@ Per ply t, for every env:
 * spatial, global = ``jq_observe`` of that seat; mask = the canonical
   legal mask ``jq_ply`` left for that seat;
 * ``policy(spatial, global, mask) -> (canonical action, log_prob, value)``
-  -- the signature of the reference's ``policy.act`` (``mask`` is bool);
+  -- the signature of the reference's ``policy.act`` (``mask`` is bool) --
+  or ``-> (logits (N, 16641), value)``: then the collector draws the action
+  itself (``policy.sample_actions``, random numbers from torch's generator);
 * with ``random_opponent`` seats 1 and 3 play a uniform legal action
   instead (gpu_collector.py:757-770);
 * the pre-action state is recorded in the compact history
@@ -52,8 +54,9 @@ import torch
 from . import _native as N
 from .env import JunqiEnvB200, _stream_ptr
 from .history import RolloutHistory
+from .policy import sample_actions
 
-Policy = Callable[[torch.Tensor, torch.Tensor, torch.Tensor], tuple[torch.Tensor, torch.Tensor, torch.Tensor]]
+Policy = Callable[[torch.Tensor, torch.Tensor, torch.Tensor], tuple[torch.Tensor, ...]]
 
 EVENT_MUTUAL = 3   # both pieces removed (rules.py Event)
 EVENT_KILLED = 4   # the moving piece was removed
@@ -97,10 +100,18 @@ class RolloutCollector:
         self._graph: torch.cuda.CUDAGraph | None = None
 
     # ------------------------------------------------------------------
-    def _act(self):
+    def _answer(self):
         env = self.env
         sp, gl = env.observe(None, seats_per_env=1)
         return self.policy(sp, gl, env.mask.view(torch.bool))
+
+    def _act(self):
+        out = self._answer()
+        if len(out) == 3:
+            return out
+        logits, v = out
+        a, lp = sample_actions(logits, self.env.mask, torch.rand(self.env.n, device=self.env.device))
+        return a, lp, v
 
     def _ply(self, t: int, ply0: int) -> None:
         env = self.env
@@ -131,7 +142,7 @@ class RolloutCollector:
         self.dones[t].copy_(term)
 
     def _final(self) -> None:
-        _, _, v = self._act()
+        v = self._answer()[-1]
         self.last_values.copy_(v.reshape(-1) * (self.env.batch["terminated"] == 0).float())
 
     def _rollout(self, ply0: int) -> None:

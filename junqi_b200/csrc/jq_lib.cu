@@ -13,6 +13,7 @@
 
 #include "jq_cellbel.cuh"
 #include "jq_hist.cuh"
+#include "jq_host.cuh"
 #include "jq_obs.cuh"
 #include "jq_ply.cuh"
 #include "jq_rules.cuh"
@@ -47,15 +48,6 @@ __global__ void rehash_kernel(jq_batch b, int mode) {
         }
         b.zobrist[e] = h;
     }
-}
-
-// Entry of the small kernels launched with programmatic dependent launch
-// (launch_pdl): let the next kernel in the stream be scheduled early, then
-// wait until the previous one has completed and its writes are visible,
-// before the first access to caller memory.
-__device__ __forceinline__ void pdl_enter() {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // compact canonical action -> world flat action (game_state.cu:2639-2685 semantics)
@@ -202,19 +194,26 @@ static DeviceState g_dev[MAX_DEV];
 static std::mutex g_mu;
 static thread_local char g_err[512] = "";
 
-static int fail(int code, const char *msg) {
+int fail(int code, const char *msg) {
     std::snprintf(g_err, sizeof g_err, "%s", msg);
     return code;
 }
-static int cuda_fail(cudaError_t err, const char *where) {
+int cuda_fail(cudaError_t err, const char *where) {
     std::snprintf(g_err, sizeof g_err, "%s: %s", where, cudaGetErrorString(err));
     return JQ_ERR_CUDA;
 }
-#define CU(call)                                                    \
-    do {                                                            \
-        cudaError_t _e = (call);                                    \
-        if (_e != cudaSuccess) return cuda_fail(_e, #call);         \
-    } while (0)
+int device_sms(int &sms) {
+    static std::atomic<int> known[MAX_DEV];
+    int d = 0;
+    CU(cudaGetDevice(&d));
+    if (d < 0 || d >= MAX_DEV) return fail(JQ_ERR_ARG, "device index out of range");
+    sms = known[d].load(std::memory_order_relaxed);
+    if (!sms) {
+        CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d));
+        known[d].store(sms, std::memory_order_relaxed);
+    }
+    return JQ_OK;
+}
 
 static int current_dev(DeviceState *&st) {
     int d = 0;
@@ -256,28 +255,6 @@ static int check_batch(const jq_batch *b) {
 
 static size_t rule_smem() { return sizeof(RuleSmem); }
 static size_t obs_smem() { return sizeof(ObsSmem); }
-
-// Programmatic dependent launch: the kernel may be scheduled while the
-// previous kernel in the stream drains (the rules kernel's slowest envs, the
-// observation kernel's last units), load its board tables into shared
-// memory, then wait (griddepcontrol.wait) for that kernel to complete
-// before touching any state.  Kernels launched this way call
-// griddepcontrol.wait before their first access to caller memory.
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
-                              Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 static int launch_rules(RuleArgs &a, cudaStream_t s) {
     DeviceState *st;
