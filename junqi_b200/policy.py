@@ -45,14 +45,17 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(i).cuda_stream, without 10 us of wrapping
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """Entry point ``name`` on the current stream of ``device``, made current for the call."""
-    fn = getattr(N.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        N.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
-    else:
+    if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            N.check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+            return _call(name, device, *args)
+    status = getattr(N.lib(), name)(*args, _raw_stream(device.index))
+    if status:
+        N.check(status, name)
 
 
 def _device(what: str, *tensors: torch.Tensor | None) -> torch.device:
@@ -122,6 +125,13 @@ def _norm_forward(shape, x2, weight, bias, eps, stats):
     return y
 
 
+def _norm_scratch(device, rows, dim):
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _norm_scratch(device, rows, dim)
+    return N.lib().jq_layer_norm_scratch_floats(rows, dim)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -142,9 +152,8 @@ class _LayerNorm(torch.autograd.Function):
         if rows:
             dy2 = _rows(dy)
             w = weight if weight is not None else bias
-            with torch.cuda.device(x2.device):
-                part = torch.empty(N.lib().jq_layer_norm_scratch_floats(rows, dim), dtype=torch.float32,
-                                   device=x2.device) if need_w or need_b else None
+            part = torch.empty(_norm_scratch(x2.device, rows, dim), dtype=torch.float32,
+                               device=x2.device) if need_w or need_b else None
             _call("jq_layer_norm_backward", x2.device, x2.data_ptr(), x2.stride(0), _ptr(weight), dy2.data_ptr(),
                   dy2.stride(0), stats.data_ptr(), rows, dim, _DTYPES[x2.dtype],
                   N.F32 if w is None else _DTYPES[w.dtype], _ptr(dx), _ptr(dw), _ptr(db), _ptr(part))
