@@ -73,14 +73,15 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*sm)[NORM_WARPS][N
 // threads apart, in groups of G places.  A row takes as few threads as hold
 // it, so its first half is inside the row for every thread, and at most the
 // last group is skipped; only rows of up to 32 places (TPR = 2) can be shorter.
-template <typename T, int VEC, int TPR>
+// FULL: every place is inside (16 tpr places), and nothing is asked.
+template <typename T, int VEC, int TPR, bool FULL>
 struct Places {
     static constexpr int G = VEC > 4 ? VEC : 4, NG = NORM_E / G, PG = G / VEC;
     f2 v[NORM_E / 2];
     static __device__ __forceinline__ bool has(int g, int groups) {  // group g of a row has places (for some thread)
-        return TPR == 2 ? g < groups : g < NG - 1 || groups == NG;
+        return FULL || (TPR == 2 ? g < groups : G == NORM_E / 2 || g < NG - 1 || groups == NG);
     }
-    static constexpr bool sure(int pack) { return TPR != 2 && pack < NORM_E / VEC / 2; }
+    static constexpr bool sure(int pack) { return FULL || (TPR != 2 && pack < NORM_E / VEC / 2); }
     __device__ __forceinline__ void load(const char *row, int t, int tpr, int dim, int groups) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -104,9 +105,9 @@ struct Places {
 };
 
 // Group g of a row, rounded and stored.
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, bool FULL>
 __device__ __forceinline__ void store_group(T *row, const f2 *v, int g, int t, int tpr, int dim) {
-    using P = Places<T, VEC, TPR>;
+    using P = Places<T, VEC, TPR, FULL>;
     alignas(16) T o[P::G];
 #pragma unroll
     for (int i = 0; i < P::G / 2; ++i) from_f2(&o[2 * i], v[i]);
@@ -170,9 +171,9 @@ struct RowStream {
 
 extern __shared__ __align__(16) char norm_ring[];
 
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, bool FULL>
 struct NormFwd {
-    using P = Places<T, VEC, TPR>;
+    using P = Places<T, VEC, TPR, FULL>;
     const NormArgs &a;
     const int t, tpr;
     f2 w[NORM_E / 2], b[NORM_E / 2];
@@ -195,7 +196,7 @@ struct NormFwd {
         row_sum<TPR>(s1, sm1, phase1);
         const float m = s1[0] * inv;
         const f2 nm = both(-m);
-        const bool whole = NORM_E * tpr == dim;
+        const bool whole = FULL || NORM_E * tpr == dim;
         f2 u = both(0.f), v = both(0.f);
 #pragma unroll
         for (int g = 0; g < P::NG; ++g)
@@ -226,7 +227,7 @@ struct NormFwd {
 #pragma unroll
                     for (int i = 0; i < P::G / 2; ++i)
                         o[i] = fma2(fma2(x.v[g * P::G / 2 + i], rr, off), w[g * P::G / 2 + i], b[g * P::G / 2 + i]);
-                    store_group<T, VEC, TPR>(y, o, g, t, tpr, dim);
+                    store_group<T, VEC, TPR, FULL>(y, o, g, t, tpr, dim);
                 }
             if (a.stats && t == 0) {
                 float *st = a.stats + (uint64_t)r * 3;
@@ -237,7 +238,7 @@ struct NormFwd {
 };
 
 // 24 warps an SM by registers.
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, bool FULL>
 __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(const NormArgs a) {
     __shared__ float sm1[TPR ? 1 : 2][NORM_WARPS][1], sm2[TPR ? 1 : 2][NORM_WARPS][2];
     pdl_enter();
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(
     const uint32_t rows = (uint32_t)a.rows, chunk = TPR ? a.chunk : 1;
     // this warp's (TPR = 0: CTA's) first row, and how far it is to its next slot's
     const uint32_t first = (TPR ? blockIdx.x * 8 + warp : blockIdx.x) * chunk, step = gridDim.x * (TPR ? 8 : 1) * chunk;
-    NormFwd<T, VEC, TPR> k{a, TPR ? lane & (TPR - 1) : (int)threadIdx.x, TPR ? TPR : (int)blockDim.x};
+    NormFwd<T, VEC, TPR, FULL> k{a, TPR ? lane & (TPR - 1) : (int)threadIdx.x, TPR ? TPR : (int)blockDim.x};
     k.sm1 = sm1, k.sm2 = sm2;
     load_weights<T, VEC>(k.w, a.w, a.wf32, 1.f, k.t, k.tpr, a.dim);
     load_weights<T, VEC>(k.b, a.b, a.wf32, 0.f, k.t, k.tpr, a.dim);
@@ -270,8 +271,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(
             __syncwarp();
             for (uint32_t q = 0; q < chunk; q += PER) {  // whole warps: every lane takes part in the shuffles
                 const uint32_t mine = q + lane / (TPR ? TPR : 32);
-                const bool valid = r0 + mine < rows;
-                k.row(xs.row(at, r0, valid ? mine : 0), r0 + mine, valid);
+                k.row(xs.row(at, r0, mine), r0 + mine, r0 + mine < rows);  // behind the last row: whatever is there, for nobody
             }
             __syncwarp();
         } else {
@@ -285,9 +285,9 @@ __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(
     copies_wait_but<0>();
 }
 
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, bool FULL>
 struct NormBwd {
-    using P = Places<T, VEC, TPR>;
+    using P = Places<T, VEC, TPR, FULL>;
     const NormArgs &a;
     const int t, tpr;
     f2 w[NORM_E / 2], aw[NORM_E / 2], ab[NORM_E / 2];
@@ -300,24 +300,22 @@ struct NormBwd {
         P x, d;
         x.load(fx, t, tpr, dim, groups);
         d.load(fy, t, tpr, dim, groups);
-        const float q = valid ? st[2] : 0.f;
-        const f2 nm = both(valid ? -st[0] : 0.f), rr = both(q), off = both(valid ? -st[1] * q : 0.f);
+        const float q = st[2];
+        const f2 nm = both(-st[0]), rr = both(q), off = both(-st[1] * q);
         f2 s = both(0.f), v = both(0.f);
         // places outside the row have dy = 0 and x = 0: a finite xh, and no part in any sum
-        if (valid) {
 #pragma unroll
-            for (int g = 0; g < P::NG; ++g)
-                if (P::has(g, groups))
+        for (int g = 0; g < P::NG; ++g)
+            if (P::has(g, groups))
 #pragma unroll
-                    for (int i = g * P::G / 2; i < (g + 1) * P::G / 2; ++i) {
-                        x.v[i] = fma2(x.v[i] + nm, rr, off);
-                        const f2 gg = d.v[i] * w[i];
-                        s = s + gg;
-                        v = fma2(gg, x.v[i], v);
-                        aw[i] = fma2(d.v[i], x.v[i], aw[i]);
-                        ab[i] = ab[i] + d.v[i];
-                    }
-        }
+                for (int i = g * P::G / 2; i < (g + 1) * P::G / 2; ++i) {
+                    x.v[i] = fma2(x.v[i] + nm, rr, off);
+                    const f2 gg = d.v[i] * w[i];
+                    s = s + gg;
+                    v = fma2(gg, x.v[i], v);
+                    aw[i] = fma2(d.v[i], x.v[i], aw[i]);
+                    ab[i] = ab[i] + d.v[i];
+                }
         if (!a.y) return;
         float sums[2] = {parts(s).x + parts(s).y, parts(v).x + parts(v).y};
         row_sum<TPR>(sums, sm, phase);
@@ -333,14 +331,14 @@ struct NormBwd {
                         const int e = g * P::G / 2 + i;
                         o[i] = fma2(x.v[e], k2, fma2(d.v[e] * w[e], rr, k1));
                     }
-                    store_group<T, VEC, TPR>(dx, o, g, t, tpr, dim);
+                    store_group<T, VEC, TPR, FULL>(dx, o, g, t, tpr, dim);
                 }
         }
     }
 };
 
 // 16 warps an SM by registers.
-template <typename T, int VEC, int TPR>
+template <typename T, int VEC, int TPR, bool FULL>
 __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(const NormArgs a) {
     constexpr int S = NORM_BWD_SLOTS, PER = 32 / (TPR ? TPR : 32);
     __shared__ float sm[TPR ? 1 : 2][NORM_WARPS][2];
@@ -348,7 +346,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
     const int lane = threadIdx.x & 31, warp = TPR ? threadIdx.x >> 5 : 0, dim = a.dim;
     const uint32_t rows = (uint32_t)a.rows, chunk = TPR ? a.chunk : 1;
     const uint32_t first = (TPR ? blockIdx.x * 8 + warp : blockIdx.x) * chunk, step = gridDim.x * (TPR ? 8 : 1) * chunk;
-    NormBwd<T, VEC, TPR> k{a, TPR ? lane & (TPR - 1) : (int)threadIdx.x, TPR ? TPR : (int)blockDim.x};
+    NormBwd<T, VEC, TPR, FULL> k{a, TPR ? lane & (TPR - 1) : (int)threadIdx.x, TPR ? TPR : (int)blockDim.x};
     k.sm = sm;
     load_weights<T, VEC>(k.w, a.w, a.wf32, 1.f, k.t, k.tpr, dim);
 #pragma unroll
@@ -363,6 +361,10 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
         if (ahead < rows) {
             char *to = ring + slot * a.slot_bytes;
             const int n = (int)min(chunk, rows - ahead);
+            if (TPR && n < (int)chunk) {  // behind the last row: zeros, which add nothing to any sum
+                for (int i = 16 * lane; i < a.slot_bytes; i += 512) *(uint4 *)(to + i) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
             xs.fetch(to, n, t, threads);
             ys.fetch(to + a.x_bytes, n, t, threads);
             const uint32_t st = (uint32_t)__cvta_generic_to_shared(to + 2 * a.x_bytes);
@@ -372,8 +374,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
         xs.skip(), ys.skip(), ahead += step;
     };
     auto row = [&](const char *at, uint32_t r0, uint32_t q, bool valid) {
-        const int mine = valid ? q : 0;
-        k.row(xs.row(at, r0, mine), ys.row(at + a.x_bytes, r0, mine), (const float *)(at + 2 * a.x_bytes) + 3 * mine, r0 + q, valid);
+        k.row(xs.row(at, r0, q), ys.row(at + a.x_bytes, r0, q), (const float *)(at + 2 * a.x_bytes) + 3 * q, r0 + q, valid);
     };
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) fetch(s);
@@ -582,7 +583,7 @@ static NormPlan norm_plan(int64_t rows, int32_t dim, int es, int vec, int sms, b
         p.kind = 1, p.chunk = 1;
         p.threads = 32 * ((dim + 32 * NORM_E - 1) / (32 * NORM_E));
         p.tpr = p.threads;
-        const int64_t cap = warps * 32 / p.threads;
+        const int64_t cap = (int64_t)sms * ((backward ? 16 : 24) * 32 / p.threads);  // whole CTAs of an SM
         p.grid = rows < cap ? rows : cap;
     }
     const int group = p.tpr * (vec > 4 ? vec : 4);
@@ -604,9 +605,9 @@ static int norm_vec(int es, int32_t dim, const void *const *ptrs, const int64_t 
     return es == 2 && (bits & 3) == 0 ? 2 : 1;
 }
 
-template <typename T, int VEC, int TPR, bool BWD>
+template <typename T, int VEC, int TPR, bool FULL, bool BWD>
 static cudaError_t norm_launch_as(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
-    auto *kernel = BWD ? norm_bwd_kernel<T, VEC, TPR> : norm_fwd_kernel<T, VEC, TPR>;
+    auto *kernel = BWD ? norm_bwd_kernel<T, VEC, TPR, FULL> : norm_fwd_kernel<T, VEC, TPR, FULL>;
     static std::atomic<uint64_t> raised{0};  // devices on which the kernel may have all of an SM's shared memory
     if (p.smem > 40 * 1024) {
         int dev = 0;
@@ -622,15 +623,22 @@ static cudaError_t norm_launch_as(const NormPlan &p, const NormArgs &a, cudaStre
     return launch_pdl(kernel, (unsigned)p.grid, (unsigned)p.threads, p.smem, s, a);
 }
 
+template <typename T, int VEC, int TPR, bool BWD>
+static cudaError_t norm_launch_tpr(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
+    constexpr bool WIDE = VEC * sizeof(T) == 16;  // rows of other widths are seldom full
+    if (WIDE && a.dim == NORM_E * p.tpr) return norm_launch_as<T, VEC, TPR, WIDE, BWD>(p, a, s);
+    return norm_launch_as<T, VEC, TPR, false, BWD>(p, a, s);
+}
+
 template <typename T, int VEC, bool BWD>
 static cudaError_t norm_launch(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
-    if (p.kind == 1) return norm_launch_as<T, VEC, 0, BWD>(p, a, s);
+    if (p.kind == 1) return norm_launch_tpr<T, VEC, 0, BWD>(p, a, s);
     switch (p.tpr) {
-        case 2: return norm_launch_as<T, VEC, 2, BWD>(p, a, s);
-        case 4: return norm_launch_as<T, VEC, 4, BWD>(p, a, s);
-        case 8: return norm_launch_as<T, VEC, 8, BWD>(p, a, s);
-        case 16: return norm_launch_as<T, VEC, 16, BWD>(p, a, s);
-        default: return norm_launch_as<T, VEC, 32, BWD>(p, a, s);
+        case 2: return norm_launch_tpr<T, VEC, 2, BWD>(p, a, s);
+        case 4: return norm_launch_tpr<T, VEC, 4, BWD>(p, a, s);
+        case 8: return norm_launch_tpr<T, VEC, 8, BWD>(p, a, s);
+        case 16: return norm_launch_tpr<T, VEC, 16, BWD>(p, a, s);
+        default: return norm_launch_tpr<T, VEC, 32, BWD>(p, a, s);
     }
 }
 

@@ -62,7 +62,15 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-template <typename T> __device__ __forceinline__ f2 to_f2(const T *v) { return make_f2(to_f(v[0]), to_f(v[1])); }
+__device__ __forceinline__ f2 to_f2(const float *v) { return make_f2(v[0], v[1]); }
+__device__ __forceinline__ f2 to_f2(const __half *v) {
+    const float2 p = __half22float2(*(const __half2 *)v);
+    return make_f2(p.x, p.y);
+}
+__device__ __forceinline__ f2 to_f2(const __nv_bfloat16 *v) {
+    const uint32_t u = *(const uint32_t *)v;  // a bfloat16 is the upper half of its float
+    return make_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
 __device__ __forceinline__ void from_f2(float *v, f2 a) {
     const float2 p = parts(a);
     v[0] = p.x, v[1] = p.y;
