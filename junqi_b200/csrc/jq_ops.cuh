@@ -121,6 +121,28 @@ __device__ __forceinline__ void copy_span(char *to, const char *from, int bytes,
     }
 }
 
+// Thread-block clusters: this CTA's place, a store into another CTA's shared
+// memory, and the barrier that makes it visible.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_store(int *mine, uint32_t rank, int v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 inline int elem_size(int dtype) { return dtype == JQ_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == JQ_F32 || dtype == JQ_F16 || dtype == JQ_BF16; }
 

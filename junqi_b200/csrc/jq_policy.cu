@@ -14,8 +14,9 @@
 // logits of the bits it found.  The packed mask (an eighth of the mask) is
 // also what the backward pass keeps: the masks that the environment and the
 // rollout history hand out are buffers that their next call overwrites.
-#include <limits.h>
 #include <math.h>
+
+#include <atomic>
 
 #include "jq_ops.cuh"
 
@@ -289,178 +290,460 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // drawn from max(p - q, 0), after the last from p: the least j whose running
 // sum exceeds r times the total.  The result is a whole number and borders
 // have to fall the same way for everybody, so everything is in 64 bits.
+//
+// The places of a game are worked on at the same time, up to 8 of them, and
+// the first that is not kept then draws: a game's chain is one place and one
+// draw, whatever its drafts.  That reads places behind the first rejection in
+// vain, but a game that goes place by place takes as long as its longest
+// chain, and the others wait for it.
+//
+// With a mask a place is one warp's: it packs the mask, lists the legal
+// actions in order, and does the rest on the list without a barrier; what
+// bounds it is the mask's bytes (with many games) or the chain of some
+// thousand cycles (with few).  Without a mask a place is a CTA's, the game a
+// cluster, and the bound is the exponentials in 64 bits.
 
-constexpr int VERIFY_THREADS = 256, VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
+constexpr int PLACES = 8;      // of a game at the same time
+constexpr int LIST = 320;      // legal actions of a place's list; with more, the packed mask is walked instead
 
 struct VerifyArgs {
     jq_drafts d;
-    int32_t words;
+    int32_t games_per_cta;  // masked: a game per warp, with no drafts; else 1
+    int32_t share;          // masked: bytes of shared memory of a warp
 };
 
-struct VerifySmem {
-    double red[2][2][VERIFY_WARPS];
-    float redf[2][2][VERIFY_WARPS];
-    double level[VERIFY_WARPS + 1];
-    int last[VERIFY_WARPS];
-    int pick;
-};
+// e^d for d <= 0 in 64 bits: d = k ln 2 / 16 + r, e^d = 2^(k / 16) e^r, from a
+// table of 16 and five terms of the series (Tang's table-driven exponential,
+// ACM TOMS 1989); |r| <= 0.0217, so the sixth is below 1.5e-13.  Below -700: 0.
+// Ten operations, where the library's function has about three times that:
+// without a mask they are the kernel's bound.  16 entries, because they lie in
+// banks of their own.
+constexpr int EXP_STEPS = 16;
+__device__ __forceinline__ double exp_table(int i) { return exp2((double)i / EXP_STEPS); }
+__device__ __forceinline__ double exp_neg(double d, const double *table) {
+    constexpr double MAGIC = 1.5 * 4503599627370496.0;  // 1.5 * 2^52: a sum's last bit is 1
+    constexpr double PER = EXP_STEPS * 1.4426950408889634, LN = 0.69314718055994531 / EXP_STEPS;
+    const double near = fma(d, PER, MAGIC);
+    const int k = __double2loint(near);
+    const double r = fma(near - MAGIC, -LN, d);
+    const double e = r * fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0);
+    const double at = table[k & (EXP_STEPS - 1)];
+    const double v = fma(at, e, at);
+    static_assert(EXP_STEPS == 16, "k >> 4");
+    const double scaled = __hiloint2double(__double2hiint(v) + ((k >> 4) << 20), __double2loint(v));
+    return d < -700.0 ? 0.0 : d == d ? scaled : d;
+}
 
 // One row of logits and what its probabilities need.
 struct Dist {
-    float m;
-    double z;
-    bool any;   // a legal place above -inf
+    double m, z, iz; // the largest logit, Z and its reciprocal
+    bool any;        // a legal place above -inf
+    __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)
+        return any ? exp_neg((double)x - m, table) : x != x ? (double)x : 0.0;
+    }
+    __device__ __forceinline__ void start(float top, bool there) {
+        any = there && top > -INFINITY;
+        m = top, z = iz = 0;
+    }
+    __device__ __forceinline__ bool broken() const { return z != z; }  // NaN or +inf at a legal place
 };
 
-__device__ __forceinline__ double weight(float x, const Dist &d) {
-    return d.any ? exp((double)x - (double)d.m) : x != x ? (double)x : 0.0;
+// What a place is, and whether its draft is kept.
+template <typename T>
+struct Place {
+    const T *x, *y;       // logits; of the draft, or NULL
+    const uint8_t *mask;
+    int act;              // the drafted action; -1 behind the last
+    bool drafted;         // i < len
+    float u;
+    Dist p, q;
+    __device__ __forceinline__ Place(const jq_drafts &d, int game, int i, int len)
+        : x((const T *)d.logits + game * d.logits_game + i * d.logits_place), y(nullptr),
+          mask(d.mask ? d.mask + game * d.mask_game + i * d.mask_place : nullptr), act(-1), drafted(i < len), u(0.f) {
+        if (drafted) {
+            act = d.drafted[(int64_t)game * d.drafts + i];
+            u = d.accept_u[(int64_t)game * d.drafts + i];
+            if (d.draft_logits) y = (const T *)d.draft_logits + game * d.draft_game + i * d.draft_place;
+        }
+        if (act >= d.actions) act = -1;
+    }
+    __device__ __forceinline__ bool broken() const { return p.broken() || q.broken(); }
+    __device__ __forceinline__ bool kept(bool legal, const double *table) const {
+        if (act < 0 || !legal || broken() || !p.any) return false;
+        const double pa = p.weight(to_f(x[act]), table) * p.iz;
+        const double qa = !y ? 1.0 : q.any ? q.weight(to_f(y[act]), table) * q.iz : 0.0;
+        return (double)u * qa < pa;
+    }
+    // the distribution that is drawn from: max(p - q, 0) while `residual`, else p
+    __device__ __forceinline__ bool has_residual() const { return drafted && (y ? q.any : act >= 0); }
+    __device__ __forceinline__ double draw_weight(int j, float xj, float yj, bool residual, const double *table) const {
+        const double pj = p.weight(xj, table) * p.iz;
+        if (!residual) return pj;
+        const double qj = y ? q.weight(yj, table) * q.iz : j == act ? 1.0 : 0.0;
+        return pj > qj ? pj - qj : 0.0;
+    }
+    __device__ __forceinline__ double draw_weight(int j, bool residual, const double *table) const {
+        return draw_weight(j, to_f(x[j]), y && residual ? to_f(y[j]) : 0.f, residual, table);
+    }
+    __device__ __forceinline__ float log_prob(int j) const {  // in 64 bits, rounded once
+        return (float)(((double)to_f(x[j]) - p.m) - log(p.z));
+    }
+};
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(ALL, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(ALL, v, o));
+    return v;
+}
+__device__ __forceinline__ double warp_scan(double v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(ALL, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
 }
 
-template <typename T, bool MASK>
-__global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs a) {
-    extern __shared__ uint32_t bits[];  // MASK: the place's packed mask
-    __shared__ VerifySmem sm;
-    pdl_enter();
+// Bits of 16 mask bytes.
+__device__ __forceinline__ uint32_t pack_block(uint4 v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        b |= ((__vminu4(w[i], 0x01010101u) * 0x01020408u) >> 24) << (4 * i);  // byte k's bit 8 k lands at 24 + k
+    return b;
+}
+
+// A row's mask in bits, in blocks of 16 bytes as they lie in memory: bit
+// (row & 15) + j for place j.  By threads t of n, eight loads in flight each.
+template <int AHEAD>
+__device__ __forceinline__ void pack_mask(uint16_t *bits, const uint8_t *row, int places, int t, int n) {
+    const int skip = (int)((uintptr_t)row & 15), blocks = (skip + places + 15) >> 4;
+    const uint8_t *first = row - skip;
+    const int k0 = skip ? 1 : 0, k1 = (skip + places) >> 4;  // whole blocks of the row
+    for (int k = k0 + t; k < k1; k += AHEAD * n) {
+        uint4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (k + i * n < k1) v[i] = *(const uint4 *)(first + 16 * (k + i * n));
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (k + i * n < k1) bits[k + i * n] = (uint16_t)pack_block(v[i]);
+    }
+    // the row's ends, a byte per thread, and the last word's upper half
+    if (t < 32) {
+        const int k = t < 16 ? 0 : blocks - 1, j = 16 * k + (t & 15) - skip;
+        const bool end = k < k0 || k >= k1;
+        const uint32_t b = __ballot_sync(ALL, end && j >= 0 && j < places && row[j] != 0);
+        if ((t & 15) == 0 && end) bits[k] = (uint16_t)(t ? b >> 16 : b);
+        if (t == 0 && (blocks & 1)) bits[blocks] = 0;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const VerifyArgs a) {
+    extern __shared__ __align__(16) char verify_smem[];
+    __shared__ double table[EXP_STEPS];
+    __shared__ int keeps[2][PLACES];
     const jq_drafts &d = a.d;
-    const int game = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n = d.actions, words = a.words;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = d.actions;
+    for (int i = threadIdx.x; i < EXP_STEPS; i += blockDim.x) table[i] = exp_table(i);
+    pdl_enter();
+    __syncthreads();
+    int *list = (int *)(verify_smem + warp * a.share);     // the legal actions in order, their logits, the draft's
+    float *lx = (float *)(list + LIST), *ly = lx + LIST;
+    uint32_t *bits = (uint32_t *)(ly + LIST);
+    const bool alone = a.games_per_cta > 1;  // a game is this warp's, and has one place
+    const int game = alone ? blockIdx.x * a.games_per_cta + warp : blockIdx.x;
+    if (game >= d.games) return;             // (alone: no barrier follows)
     int len = d.lengths ? d.lengths[game] : d.drafts;
     len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
     int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
     float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
-    int buf = 0;
-    for (int i = 0;; ++i) {
-        const T *x = (const T *)d.logits + game * d.logits_game + i * d.logits_place;
-        const T *y = d.draft_logits && i < len
-                         ? (const T *)d.draft_logits + game * d.draft_game + i * d.draft_place : nullptr;
-        const uint8_t *mask = MASK ? d.mask + game * d.mask_game + i * d.mask_place : nullptr;
-        __syncthreads();  // the last place's bits have been read
-        if (MASK) {
-            for (int w = tid; w < words; w += VERIFY_THREADS) bits[w] = legal_word(mask, n, w);
-        }
-        // every legal place of this thread: words tid, tid + 256, ..., or with no mask places tid, tid + 256, ...
+    for (int base = 0, round = 0;; base += warps, round ^= 1) {
+        const int i = alone ? 0 : base + warp;
+        const bool active = i <= len;
+        bool kept = false;
+        Place<T> at(d, game, active ? i : len, len);
+        int count = 0, lo = 0, hi = 0;
+        const int skip = (int)((uintptr_t)at.mask & 15), words = (skip + n + 31) >> 5;
+        const int share = (words + 31) >> 5, w0 = min(words, lane * share), w1 = min(words, w0 + share);
+        // this lane's legal actions, consecutive ones, with their logits: of the list, or of the packed mask
         auto each = [&](auto &&f) {
-            if (MASK) {
-                for (int w = tid; w < words; w += VERIFY_THREADS)
-                    for (uint32_t b = bits[w]; b; b &= b - 1) f(32 * w + __ffs(b) - 1);
+            if (count <= LIST) {
+                for (int k = lo; k < hi; ++k) f(list[k], lx[k], ly[k]);
             } else {
-#pragma unroll 4
-                for (int j = tid; j < n; j += VERIFY_THREADS) f(j);
+                for (int w = w0; w < w1; ++w)
+                    for (uint32_t b = bits[w]; b; b &= b - 1) {
+                        const int j = 32 * w + __ffs(b) - 1 - skip;
+                        f(j, to_f(at.x[j]), at.y ? to_f(at.y[j]) : 0.f);
+                    }
             }
         };
-        float mx = -INFINITY, my = -INFINITY;
-        each([&](int j) {
-            mx = fmaxf(mx, to_f(x[j]));
-            if (y) my = fmaxf(my, to_f(y[j]));
-        });
+        if (active) {
+            __syncwarp();
+            pack_mask<8>((uint16_t *)bits, at.mask, n, lane, 32);
+            __syncwarp();
+            int mine = 0;
+            for (int w = w0; w < w1; ++w) mine += __popc(bits[w]);
+            int before = mine;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, o));
-            my = fmaxf(my, __shfl_xor_sync(ALL, my, o));
-        }
-        if (lane == 0) sm.redf[buf][0][warp] = mx, sm.redf[buf][1][warp] = my;
-        __syncthreads();
-        Dist p{sm.redf[buf][0][0], 0, false}, q{sm.redf[buf][1][0], 0, false};
-        for (int k = 1; k < VERIFY_WARPS; ++k) p.m = fmaxf(p.m, sm.redf[buf][0][k]), q.m = fmaxf(q.m, sm.redf[buf][1][k]);
-        p.any = p.m > -INFINITY, q.any = y && q.m > -INFINITY;
-        double zx = 0, zy = 0;
-        each([&](int j) {
-            zx += weight(to_f(x[j]), p);
-            if (y) zy += weight(to_f(y[j]), q);
-        });
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            zx += __shfl_xor_sync(ALL, zx, o);
-            zy += __shfl_xor_sync(ALL, zy, o);
-        }
-        if (lane == 0) sm.red[buf][0][warp] = zx, sm.red[buf][1][warp] = zy;
-        __syncthreads();
-        for (int k = 0; k < VERIFY_WARPS; ++k) p.z += sm.red[buf][0][k], q.z += sm.red[buf][1][k];
-        buf ^= 1;
-        const bool broken = p.z != p.z || q.z != q.z;  // NaN or +inf at a legal place: no distribution
-        const double logz = log(p.z);
-        const int act = i < len ? d.drafted[(int64_t)game * d.drafts + i] : -1;
-        if (act >= 0 && act < n && !broken && is_legal(nullptr, MASK ? bits : nullptr, act) && p.any) {
-            const float xa = to_f(x[act]);
-            const double pa = weight(xa, p) / p.z;
-            const double qa = !d.draft_logits ? 1.0 : q.any ? weight(to_f(y[act]), q) / q.z : 0.0;
-            if ((double)d.accept_u[(int64_t)game * d.drafts + i] * qa < pa) {
-                if (tid == 0) out[i] = act, out_lp[i] = (float)(((double)xa - (double)p.m) - logz);
-                continue;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(ALL, before, o);
+                if (lane >= o) before += u;
             }
-        }
-        // place i is not kept (or i == len): draw here, and be done
-        const bool bare = !d.draft_logits && i < len;  // q is one-hot at the drafted action
-        const bool use_q = i < len && (bare ? act >= 0 && act < n : q.any);
-        auto w_of = [&](int j, bool residual) {
-            const double pj = weight(to_f(x[j]), p) / p.z;
-            if (!residual) return pj;
-            const double qj = bare ? (j == act ? 1.0 : 0.0) : weight(to_f(y[j]), q) / q.z;
-            return pj > qj ? pj - qj : 0.0;
-        };
-        int next = -1;
-        if (p.any && !broken) {
-            float rf = d.sample_u[game];
-            const double r = rf > 0.f ? (double)rf : 0.0;
-            // a thread's share is consecutive, so that running sums follow the order of the actions
-            const int units = MASK ? words : n, share = (units + VERIFY_THREADS - 1) / VERIFY_THREADS;
-            const int u0 = min(units, tid * share), u1 = min(units, u0 + share);
-            for (int pass = use_q ? 0 : 1; pass < 2; ++pass) {
-                const bool residual = pass == 0;
-                auto walk = [&](auto &&f) {
-                    for (int u = u0; u < u1; ++u) {
-                        if (MASK) {
-                            for (uint32_t b = bits[u]; b; b &= b - 1) f(32 * u + __ffs(b) - 1);
-                        } else {
-                            f(u);
+            count = __shfl_sync(ALL, before, 31);
+            before -= mine;
+            if (count <= LIST) {
+                for (int w = w0; w < w1; ++w)
+                    for (uint32_t b = bits[w]; b; b &= b - 1) list[before++] = 32 * w + __ffs(b) - 1 - skip;
+                const int per = (count + 31) >> 5;
+                lo = min(count, lane * per), hi = min(count, lo + per);
+                __syncwarp();
+                for (int k0 = 0; k0 < count; k0 += 128) {  // four scattered logits of each in flight
+                    float vx[4], vy[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = k0 + 32 * i + lane;
+                        if (k < count) {
+                            vx[i] = to_f(at.x[list[k]]);
+                            if (at.y) vy[i] = to_f(at.y[list[k]]);
                         }
                     }
-                };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = k0 + 32 * i + lane;
+                        if (k < count) lx[k] = vx[i], ly[k] = at.y ? vy[i] : 0.f;
+                    }
+                }
+                __syncwarp();
+            }
+            float mx = -INFINITY, my = -INFINITY;
+            each([&](int, float x, float y) { mx = fmaxf(mx, x), my = fmaxf(my, y); });
+            at.p.start(warp_max(mx), true);
+            at.q.start(warp_max(my), at.y != nullptr);
+            double zx = 0, zy = 0;
+            each([&](int, float x, float y) {
+                zx += at.p.weight(x, table);
+                if (at.y) zy += at.q.weight(y, table);
+            });
+            at.p.z = warp_sum(zx), at.q.z = warp_sum(zy);
+            at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
+            const int b = at.act + skip;
+            kept = at.kept(at.act >= 0 && ((bits[b >> 5] >> (b & 31)) & 1), table);
+        }
+        int first = alone ? 0 : warps;  // the first place of this round that is not kept
+        if (!alone) {
+            if (lane == 0) keeps[round][warp] = kept;
+            __syncthreads();
+            for (int k = warps - 1; k >= 0; --k)
+                if (!keeps[round][k]) first = k;
+            if (kept && warp < first && lane == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
+            if (first == warps) continue;
+            if (warp != first) return;
+        }
+        int next = -1;
+        if (at.p.any && !at.broken()) {
+            const float rf = d.sample_u[game];
+            const double r = rf > 0.f ? (double)rf : 0.0;
+            for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
+                const bool residual = pass == 0;
                 double part = 0;
-                walk([&](int j) { part += w_of(j, residual); });
-                double inc = part;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double v = __shfl_up_sync(ALL, inc, o);
-                    if (lane >= o) inc += v;
-                }
-                __syncthreads();
-                if (lane == 31) sm.level[warp] = inc;
-                if (tid == 0) sm.pick = INT_MAX;
-                __syncthreads();
-                double before = 0, total = 0;
-                for (int k = 0; k < VERIFY_WARPS; ++k) {
-                    if (k < warp) before += sm.level[k];
-                    total += sm.level[k];
-                }
+                each([&](int j, float x, float y) { part += at.draw_weight(j, x, y, residual, table); });
+                const double above = warp_scan(part, lane), total = __shfl_sync(ALL, above, 31);
                 if (residual && !(total > RESIDUAL_MIN)) continue;
-                double lo = __shfl_up_sync(ALL, inc, 1);
-                lo = before + (lane ? lo : 0.0);
-                const double hi = before + inc, target = r * total;
-                int last = -1;
-                if (part > 0) {
-                    double run = lo;
+                const double up = __shfl_up_sync(ALL, above, 1), below = lane ? up : 0.0, target = r * total;
+                // the first lane whose running sum is above the point; with none, the last that has weight
+                const unsigned cross = __ballot_sync(ALL, part > 0 && above > target), some = __ballot_sync(ALL, part > 0);
+                const int who = cross ? __ffs(cross) - 1 : 31 - __clz(some);
+                if (lane == who) {
+                    double run = below;
                     bool crossed = false;
-                    walk([&](int j) {
-                        const double w = w_of(j, residual);
+                    each([&](int j, float x, float y) {
+                        const double w = at.draw_weight(j, x, y, residual, table);
                         run += w;
-                        if (w > 0) {
-                            if (!crossed) last = j;
-                            if (run > target) crossed = true;
-                        }
+                        if (w > 0 && !crossed) next = j, crossed = run > target;
                     });
-                    if (lo <= target && hi > target) atomicMin(&sm.pick, last);
+                }
+                next = __shfl_sync(ALL, next, who);
+                break;
+            }
+        }
+        if (lane == 0) {
+            d.accepted[game] = i;
+            out[i] = next;
+            out_lp[i] = next >= 0 ? at.log_prob(next) : at.broken() ? __int_as_float(0x7fc00000) : 0.f;
+        }
+        for (int k = i + 1 + lane; k <= d.drafts; k += 32) out[k] = -1, out_lp[k] = 0.f;
+        return;
+    }
+}
+
+// Without a mask: a cluster per game, a CTA per place.
+constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32;
+
+// Every logit of a row, by the CTA: 8 bytes a load, the ends one by one.
+template <typename T, typename F>
+__device__ __forceinline__ void dense_each(const T *x, int n, int tid, F &&f) {
+    constexpr int VEC = 8 / sizeof(T);
+    const int head = min(n, (int)((8 - ((uintptr_t)x & 7)) & 7) / (int)sizeof(T)), packs = (n - head) / VEC;
+    const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
+    int k = tid;
+    for (; k + 3 * DENSE_THREADS < packs; k += 4 * DENSE_THREADS) {
+        Pack<T, VEC> p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] = px[k + u * DENSE_THREADS];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f(to_f(p[u].v[i]));
+    }
+    for (; k < packs; k += DENSE_THREADS) {
+        const Pack<T, VEC> p = px[k];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f(to_f(p.v[i]));
+    }
+    const int rest = n - packs * VEC;  // before the first pack and behind the last
+    if (tid < rest) f(to_f(x[tid < head ? tid : tid + packs * VEC]));
+}
+
+// Sum of exp(x - m) over this thread's logits of a row.
+template <typename T>
+__device__ __forceinline__ double dense_sum(const T *x, int n, int tid, const Dist &d, const double *table) {
+    double z = 0;
+    if (d.any)
+        dense_each(x, n, tid, [&](float v) { z += exp_neg((double)v - d.m, table); });
+    else
+        dense_each(x, n, tid, [&](float v) { z += v != v ? (double)v : 0.0; });
+    return z;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(DENSE_THREADS) verify_dense_kernel(const VerifyArgs a) {
+    __shared__ double table[EXP_STEPS];
+    __shared__ double sums[2][DENSE_WARPS], level[DENSE_WARPS];
+    __shared__ float tops[2][DENSE_WARPS];
+    __shared__ int keeps[2][PLACES], pick;
+    const jq_drafts &d = a.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = d.actions;
+    const int rank = (int)cluster_rank(), ranks = (int)cluster_size(), game = blockIdx.x / ranks;
+    for (int i = tid; i < EXP_STEPS; i += DENSE_THREADS) table[i] = exp_table(i);
+    pdl_enter();
+    cluster_sync();  // the game's CTAs have all started: their shared memory may be written
+    int len = d.lengths ? d.lengths[game] : d.drafts;
+    len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
+    int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
+    float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
+    for (int base = 0, round = 0;; base += ranks, round ^= 1) {
+        const int i = base + rank;
+        const bool active = i <= len;
+        bool kept = false;
+        Place<T> at(d, game, active ? i : len, len);
+        if (active) {
+            float mx = -INFINITY, my = -INFINITY;
+            dense_each(at.x, n, tid, [&](float v) { mx = fmaxf(mx, v); });
+            if (at.y) dense_each(at.y, n, tid, [&](float v) { my = fmaxf(my, v); });
+            mx = warp_max(mx), my = warp_max(my);
+            if (lane == 0) tops[0][warp] = mx, tops[1][warp] = my;
+            __syncthreads();
+            for (int k = 0; k < DENSE_WARPS; ++k) mx = fmaxf(mx, tops[0][k]), my = fmaxf(my, tops[1][k]);
+            at.p.start(mx, true), at.q.start(my, at.y != nullptr);
+            double zx = dense_sum(at.x, n, tid, at.p, table), zy = at.y ? dense_sum(at.y, n, tid, at.q, table) : 0.0;
+            zx = warp_sum(zx), zy = warp_sum(zy);
+            if (lane == 0) sums[0][warp] = zx, sums[1][warp] = zy;
+            __syncthreads();
+            for (int k = 0; k < DENSE_WARPS; ++k) at.p.z += sums[0][k], at.q.z += sums[1][k];
+            at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
+            kept = at.kept(true, table);
+        }
+        if (tid < ranks) cluster_store(&keeps[round][rank], tid, (int)kept);  // to every CTA of the game
+        cluster_sync();
+        int first = ranks;
+        for (int k = ranks - 1; k >= 0; --k)
+            if (!keeps[round][k]) first = k;
+        if (kept && rank < first && tid == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
+        if (first == ranks) continue;
+        if (rank != first) return;
+        int next = -1;
+        if (at.p.any && !at.broken()) {
+            const float rf = d.sample_u[game];
+            const double r = rf > 0.f ? (double)rf : 0.0;
+            for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
+                const bool residual = pass == 0;
+                // the place of the point: an eighth of the row, of that an eighth, and so on, each warp a share
+                int from = 0, to = n;
+                double target = 0, below = 0;
+                bool none = false, wide = true;  // wide: the whole row, whose total is not known yet
+                while (to - from > 32) {
+                    const int share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
+                    const int w0 = min(to, from + warp * share), w1 = min(to, w0 + share);
+                    double part = 0;
+                    if (residual && at.y) {
+#pragma unroll 4
+                        for (int j = w0 + lane; j < w1; j += 32) {
+                            const double pj = exp_neg((double)to_f(at.x[j]) - at.p.m, table) * at.p.iz;
+                            const double qj = exp_neg((double)to_f(at.y[j]) - at.q.m, table) * at.q.iz;
+                            part += fmax(pj - qj, 0.0);
+                        }
+                    } else {
+#pragma unroll 4
+                        for (int j = w0 + lane; j < w1; j += 32) part += at.draw_weight(j, residual, table);
+                    }
+                    part = warp_sum(part);
+                    __syncthreads();
+                    if (lane == 0) level[warp] = part;
+                    __syncthreads();
+                    if (wide) {
+                        double total = 0;
+                        for (int k = 0; k < DENSE_WARPS; ++k) total += level[k];
+                        none = residual && !(total > RESIDUAL_MIN);
+                        target = r * total;
+                        wide = false;
+                    }
+                    if (none) break;
+                    // the first share whose running sum is above the point; with none, the last that has weight
+                    double run = below;
+                    int who = -1, last = 0;
+                    double at_last = below;
+                    for (int k = 0; k < DENSE_WARPS; ++k) {
+                        if (level[k] > 0) {
+                            last = k, at_last = run;
+                            if (run + level[k] > target) {
+                                who = k;
+                                break;
+                            }
+                        }
+                        run += level[k];
+                    }
+                    if (who < 0) who = last;
+                    below = at_last;
+                    const int f = min(to, from + who * share);
+                    to = min(to, f + share), from = f;
+                }
+                if (none) continue;
+                if (warp == 0) {
+                    const int j = from + lane;
+                    const double w = j < to ? at.draw_weight(j, residual, table) : 0.0;
+                    const double above = warp_scan(w, lane);
+                    if (wide) {  // a row of at most 32 places
+                        const double total = __shfl_sync(ALL, above, 31);
+                        none = residual && !(total > RESIDUAL_MIN);
+                        target = r * total;
+                    }
+                    const unsigned cross = __ballot_sync(ALL, w > 0 && below + above > target), some = __ballot_sync(ALL, w > 0);
+                    if (lane == 0) pick = none ? -2 : from + (cross ? __ffs(cross) - 1 : 31 - __clz(some));
                 }
                 __syncthreads();
-                next = sm.pick;
-                if (next == INT_MAX) {  // the point is at the total or beyond: the last place with weight
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(ALL, last, o));
-                    if (lane == 0) sm.last[warp] = last;
+                next = pick;
+                if (next == -2) {
                     __syncthreads();
-                    next = -1;
-                    for (int k = 0; k < VERIFY_WARPS; ++k) next = max(next, sm.last[k]);
+                    continue;
                 }
                 break;
             }
@@ -468,12 +751,52 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
         if (tid == 0) {
             d.accepted[game] = i;
             out[i] = next;
-            out_lp[i] = next >= 0 ? (float)(((double)to_f(x[next]) - (double)p.m) - logz)
-                                  : broken ? __int_as_float(0x7fc00000) : 0.f;
+            out_lp[i] = next >= 0 ? at.log_prob(next) : at.broken() ? __int_as_float(0x7fc00000) : 0.f;
         }
-        for (int k = i + 1 + tid; k <= d.drafts; k += VERIFY_THREADS) out[k] = -1, out_lp[k] = 0.f;
+        for (int k = i + 1 + tid; k <= d.drafts; k += DENSE_THREADS) out[k] = -1, out_lp[k] = 0.f;
         return;
     }
+}
+
+template <typename T>
+static int verify_launch(const jq_drafts &d, cudaStream_t s) {
+    VerifyArgs a{d, 1, 0};
+    const int places = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
+    if (!d.mask) {
+        if ((int64_t)d.games * places > INT32_MAX) return fail(JQ_ERR_CAPACITY, "drafts: too many games for one call");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)d.games * places);
+        cfg.blockDim = dim3(DENSE_THREADS);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = places, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr, cfg.numAttrs = 2;
+        CU(cudaLaunchKernelEx(&cfg, verify_dense_kernel<T>, a));
+        return JQ_OK;
+    }
+    a.share = 4 * (3 * LIST + (d.actions + 15 + 31) / 32 + 1);
+    a.share = (a.share + 15) & ~15;
+    int warps = places;
+    if (d.drafts == 0) warps = a.games_per_cta = 4;
+    while (warps > 1 && (size_t)warps * a.share > 200 * 1024) --warps;
+    if (d.drafts == 0) a.games_per_cta = warps;
+    const size_t smem = (size_t)warps * a.share;
+    if (smem > 40 * 1024) {
+        static std::atomic<uint64_t> raised{0};
+        int dev = 0;
+        CU(cudaGetDevice(&dev));
+        const uint64_t bit = 1ull << (dev & 63);
+        if (!(raised.load(std::memory_order_relaxed) & bit)) {
+            CU(cudaFuncSetAttribute(verify_masked_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 210 * 1024));
+            raised.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    const unsigned g = (unsigned)((d.games + a.games_per_cta - 1) / a.games_per_cta);
+    CU(launch_pdl(verify_masked_kernel<T>, g, 32 * warps, smem, s, a));
+    return JQ_OK;
 }
 
 }  // namespace jq
@@ -561,21 +884,10 @@ int jq_verify_drafts(const jq_drafts *d, void *stream) {
          (uintptr_t)d->accepted | (uintptr_t)d->out_actions | (uintptr_t)d->log_probs) & 3 ||
         (uintptr_t)d->draft_logits & (elem_size(d->dtype) - 1))
         return fail(JQ_ERR_ARG, "drafts: an array is not aligned to its elements");
-    VerifyArgs a{*d, (d->actions + 31) / 32};
-    const bool masked = d->mask != nullptr;
-    const size_t smem = masked ? 4 * (size_t)a.words : 0;
-    const unsigned g = (unsigned)d->games;
     cudaStream_t s = (cudaStream_t)stream;
-    if (d->dtype == JQ_F32)
-        CU(masked ? launch_pdl(verify_kernel<float, true>, g, VERIFY_THREADS, smem, s, a)
-                  : launch_pdl(verify_kernel<float, false>, g, VERIFY_THREADS, smem, s, a));
-    else if (d->dtype == JQ_F16)
-        CU(masked ? launch_pdl(verify_kernel<__half, true>, g, VERIFY_THREADS, smem, s, a)
-                  : launch_pdl(verify_kernel<__half, false>, g, VERIFY_THREADS, smem, s, a));
-    else
-        CU(masked ? launch_pdl(verify_kernel<__nv_bfloat16, true>, g, VERIFY_THREADS, smem, s, a)
-                  : launch_pdl(verify_kernel<__nv_bfloat16, false>, g, VERIFY_THREADS, smem, s, a));
-    return JQ_OK;
+    if (d->dtype == JQ_F32) return verify_launch<float>(*d, s);
+    if (d->dtype == JQ_F16) return verify_launch<__half>(*d, s);
+    return verify_launch<__nv_bfloat16>(*d, s);
 }
 
 }  // extern "C"
