@@ -297,11 +297,11 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // vain, but a game that goes place by place takes as long as its longest
 // chain, and the others wait for it.
 //
-// With a mask a place is one warp's: it packs the mask, lists the legal
-// actions in order, and does the rest on the list without a barrier; what
-// bounds it is the mask's bytes (with many games) or the chain of some
-// thousand cycles (with few).  Without a mask a place is a CTA's, the game a
-// cluster, and the bound is the exponentials in 64 bits.
+// That is with a mask, where a place is one warp's: it packs the mask, lists
+// the legal actions in order, and does the rest on the list without a barrier;
+// what bounds it is the mask's bytes (with many games) or the chain of some
+// thousand cycles (with few).  Without a mask the bound is the exponentials in
+// 64 bits (verify_dense_kernel).
 
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
 constexpr int PLACES = 8;      // of a game at the same time
@@ -410,40 +410,61 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
     return v;
 }
 
-// Bits of 16 mask bytes.
+// Bits of 16 mask bytes: bytes of 0 and 1 are dot products with powers of two.
 __device__ __forceinline__ uint32_t pack_block(uint4 v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t b = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        b |= ((__vminu4(w[i], 0x01010101u) * 0x01020408u) >> 24) << (4 * i);  // byte k's bit 8 k lands at 24 + k
-    return b;
+    if ((v.x | v.y | v.z | v.w) & 0xfefefefeu)  // other truth values
+        v = make_uint4(__vminu4(v.x, 0x01010101u), __vminu4(v.y, 0x01010101u), __vminu4(v.z, 0x01010101u), __vminu4(v.w, 0x01010101u));
+    const uint32_t lo = __dp4a(v.y, 0x80402010u, __dp4a(v.x, 0x08040201u, 0u));
+    const uint32_t hi = __dp4a(v.w, 0x80402010u, __dp4a(v.z, 0x08040201u, 0u));
+    return lo | hi << 8;
 }
 
 // A row's mask in bits, in blocks of 16 bytes as they lie in memory: bit
-// (row & 15) + j for place j.  By threads t of n, eight loads in flight each.
-template <int AHEAD>
-__device__ __forceinline__ void pack_mask(uint16_t *bits, const uint8_t *row, int places, int t, int n) {
+// (row & 15) + j for place j; by a warp, eight loads in flight a lane.  Blocks
+// with legal places go to `found` too, in order, as block << 16 | bits, as
+// long as there are at most `most`; their number is returned.
+__device__ __forceinline__ int pack_mask(uint16_t *bits, uint32_t *found, int most, const uint8_t *row, int places, int lane) {
+    constexpr int AHEAD = 8;
     const int skip = (int)((uintptr_t)row & 15), blocks = (skip + places + 15) >> 4;
     const uint8_t *first = row - skip;
     const int k0 = skip ? 1 : 0, k1 = (skip + places) >> 4;  // whole blocks of the row
-    for (int k = k0 + t; k < k1; k += AHEAD * n) {
+    // the row's ends, a byte per lane, and the last word's upper half
+    const int ke = lane < 16 ? 0 : blocks - 1, je = 16 * ke + (lane & 15) - skip;
+    const bool end = lane < 16 ? k0 > 0 || k1 == 0 : k1 < blocks && blocks > 1;
+    const uint32_t ends = __ballot_sync(ALL, end && je >= 0 && je < places && row[je] != 0);
+    if ((lane & 15) == 0 && end) bits[ke] = (uint16_t)(lane ? ends >> 16 : ends);
+    if (lane == 0 && (blocks & 1)) bits[blocks] = 0;
+    int n = 0;
+    if (ends & 0xffff) {
+        if (lane == 0) found[0] = ends & 0xffff;
+        n = 1;
+    }
+    for (int b0 = k0; b0 < k1; b0 += 32 * AHEAD) {
         uint4 v[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (k + i * n < k1) v[i] = *(const uint4 *)(first + 16 * (k + i * n));
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = b0 + 32 * i + lane;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (k < k1) v[i] = *(const uint4 *)(first + 16 * k);
+        }
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (k + i * n < k1) bits[k + i * n] = (uint16_t)pack_block(v[i]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = b0 + 32 * i + lane;
+            const uint32_t b = pack_block(v[i]);
+            if (k < k1) bits[k] = (uint16_t)b;
+            const uint32_t some = __ballot_sync(ALL, b != 0);
+            if (b) {
+                const int at = n + __popc(some & ((1u << lane) - 1));
+                if (at < most) found[at] = (uint32_t)k << 16 | b;
+            }
+            n += __popc(some);
+        }
     }
-    // the row's ends, a byte per thread, and the last word's upper half
-    if (t < 32) {
-        const int k = t < 16 ? 0 : blocks - 1, j = 16 * k + (t & 15) - skip;
-        const bool end = k < k0 || k >= k1;
-        const uint32_t b = __ballot_sync(ALL, end && j >= 0 && j < places && row[j] != 0);
-        if ((t & 15) == 0 && end) bits[k] = (uint16_t)(t ? b >> 16 : b);
-        if (t == 0 && (blocks & 1)) bits[blocks] = 0;
+    if (ends >> 16) {
+        if (lane == 0 && n < most) found[n] = (uint32_t)(blocks - 1) << 16 | ends >> 16;
+        ++n;
     }
+    return n;
 }
 
 template <typename T>
@@ -488,21 +509,30 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
         };
         if (active) {
             __syncwarp();
-            pack_mask<8>((uint16_t *)bits, at.mask, n, lane, 32);
+            uint32_t *found = (uint32_t *)lx;
+            const int blocks = pack_mask((uint16_t *)bits, found, LIST, at.mask, n, lane);
             __syncwarp();
-            int mine = 0;
-            for (int w = w0; w < w1; ++w) mine += __popc(bits[w]);
-            int before = mine;
+            // this lane's legal places: of its share of the blocks that have some, or of the words
+            const bool few = blocks <= LIST;
+            const int per_lane = (blocks + 31) >> 5, e0 = min(blocks, lane * per_lane), e1 = min(blocks, e0 + per_lane);
+            int before = 0;
+            if (few)
+                for (int e = e0; e < e1; ++e) before += __popc(found[e] & 0xffff);
+            else
+                for (int w = w0; w < w1; ++w) before += __popc(bits[w]);
+            const int own = before;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(ALL, before, o);
                 if (lane >= o) before += u;
             }
             count = __shfl_sync(ALL, before, 31);
-            before -= mine;
+            before -= own;
             if (count <= LIST) {
-                for (int w = w0; w < w1; ++w)
-                    for (uint32_t b = bits[w]; b; b &= b - 1) list[before++] = 32 * w + __ffs(b) - 1 - skip;
+                for (int e = e0; e < e1; ++e) {
+                    const int j0 = (int)(found[e] >> 16) * 16 - skip;
+                    for (uint32_t b = found[e] & 0xffff; b; b &= b - 1) list[before++] = j0 + __ffs(b) - 1;
+                }
                 const int per = (count + 31) >> 5;
                 lo = min(count, lane * per), hi = min(count, lo + per);
                 __syncwarp();
@@ -585,10 +615,12 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
     }
 }
 
-// Without a mask: a cluster per game, a CTA per place.
-constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32;
+// Without a mask: a cluster per game, each CTA a consecutive share of every
+// row.  Place by place, since a place is enough work for the whole cluster:
+// no row behind the first rejection is read.
+constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32, DENSE_CTAS = 8;
 
-// Every logit of a row, by the CTA: 8 bytes a load, the ends one by one.
+// Every logit of x[0, n), by the CTA: 8 bytes a load, the ends one by one.
 template <typename T, typename F>
 __device__ __forceinline__ void dense_each(const T *x, int n, int tid, F &&f) {
     constexpr int VEC = 8 / sizeof(T);
@@ -613,7 +645,7 @@ __device__ __forceinline__ void dense_each(const T *x, int n, int tid, F &&f) {
     if (tid < rest) f(to_f(x[tid < head ? tid : tid + packs * VEC]));
 }
 
-// Sum of exp(x - m) over this thread's logits of a row.
+// Sum of exp(x - m) over this thread's logits of x[0, n).
 template <typename T>
 __device__ __forceinline__ double dense_sum(const T *x, int n, int tid, const Dist &d, const double *table) {
     double z = 0;
@@ -624,130 +656,154 @@ __device__ __forceinline__ double dense_sum(const T *x, int n, int tid, const Di
     return z;
 }
 
+struct DenseSmem {
+    double table[EXP_STEPS];
+    double sums[2][DENSE_WARPS], level[DENSE_WARPS];
+    float tops[2][DENSE_WARPS];
+    double told[2][DENSE_CTAS][4];  // what the game's CTAs tell each other: two rounds' m, Z of the target, m, Z of the draft
+    int pick;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(DENSE_THREADS) verify_dense_kernel(const VerifyArgs a) {
-    __shared__ double table[EXP_STEPS];
-    __shared__ double sums[2][DENSE_WARPS], level[DENSE_WARPS];
-    __shared__ float tops[2][DENSE_WARPS];
-    __shared__ int keeps[2][PLACES], pick;
+__global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const VerifyArgs a) {
+    __shared__ DenseSmem sm;
     const jq_drafts &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = d.actions;
     const int rank = (int)cluster_rank(), ranks = (int)cluster_size(), game = blockIdx.x / ranks;
-    for (int i = tid; i < EXP_STEPS; i += DENSE_THREADS) table[i] = exp_table(i);
+    if (tid < EXP_STEPS) sm.table[tid] = exp_table(tid);
+    const double *table = sm.table;
     pdl_enter();
     cluster_sync();  // the game's CTAs have all started: their shared memory may be written
     int len = d.lengths ? d.lengths[game] : d.drafts;
     len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
     int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
     float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
-    for (int base = 0, round = 0;; base += ranks, round ^= 1) {
-        const int i = base + rank;
-        const bool active = i <= len;
-        bool kept = false;
-        Place<T> at(d, game, active ? i : len, len);
-        if (active) {
+    const int all = ((n + ranks - 1) / ranks + 31) & ~31, s0 = min(n, rank * all), s1 = min(n, s0 + all);
+    int round = 0;
+    // `v` (of thread 0) of every CTA to every CTA, as told[round][rank][at]
+    auto tell = [&](int at, double v) {
+        for (int k = 0; k < ranks; ++k) cluster_store(&sm.told[round][rank][at], k, v);
+    };
+    for (int i = 0;; ++i) {
+        Place<T> at(d, game, i, len);
+        {
             float mx = -INFINITY, my = -INFINITY;
-            dense_each(at.x, n, tid, [&](float v) { mx = fmaxf(mx, v); });
-            if (at.y) dense_each(at.y, n, tid, [&](float v) { my = fmaxf(my, v); });
+            dense_each(at.x + s0, s1 - s0, tid, [&](float v) { mx = fmaxf(mx, v); });
+            if (at.y) dense_each(at.y + s0, s1 - s0, tid, [&](float v) { my = fmaxf(my, v); });
             mx = warp_max(mx), my = warp_max(my);
-            if (lane == 0) tops[0][warp] = mx, tops[1][warp] = my;
             __syncthreads();
-            for (int k = 0; k < DENSE_WARPS; ++k) mx = fmaxf(mx, tops[0][k]), my = fmaxf(my, tops[1][k]);
+            if (lane == 0) sm.tops[0][warp] = mx, sm.tops[1][warp] = my;
+            __syncthreads();
+            for (int k = 0; k < DENSE_WARPS; ++k) mx = fmaxf(mx, sm.tops[0][k]), my = fmaxf(my, sm.tops[1][k]);
             at.p.start(mx, true), at.q.start(my, at.y != nullptr);
-            double zx = dense_sum(at.x, n, tid, at.p, table), zy = at.y ? dense_sum(at.y, n, tid, at.q, table) : 0.0;
+            double zx = dense_sum(at.x + s0, s1 - s0, tid, at.p, table);
+            double zy = at.y ? dense_sum(at.y + s0, s1 - s0, tid, at.q, table) : 0.0;
             zx = warp_sum(zx), zy = warp_sum(zy);
-            if (lane == 0) sums[0][warp] = zx, sums[1][warp] = zy;
+            if (lane == 0) sm.sums[0][warp] = zx, sm.sums[1][warp] = zy;
             __syncthreads();
-            for (int k = 0; k < DENSE_WARPS; ++k) at.p.z += sums[0][k], at.q.z += sums[1][k];
+            for (int k = 0; k < DENSE_WARPS; ++k) at.p.z += sm.sums[0][k], at.q.z += sm.sums[1][k];
+            if (ranks > 1) {
+                if (tid == 0) tell(0, at.p.m), tell(1, at.p.z), tell(2, at.q.m), tell(3, at.q.z);
+                cluster_sync();
+                double m[2] = {-INFINITY, -INFINITY}, z[2] = {0, 0};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    for (int k = 0; k < ranks; ++k) m[h] = fmax(m[h], sm.told[round][k][2 * h]);
+                    for (int k = 0; k < ranks; ++k) {
+                        const double mk = sm.told[round][k][2 * h], zk = sm.told[round][k][2 * h + 1];
+                        z[h] += mk > -INFINITY ? zk * exp_neg(mk - m[h], table) : zk;  // (a share of -inf has Z = 0 or NaN)
+                    }
+                }
+                round ^= 1;
+                at.p.start((float)m[0], true), at.q.start((float)m[1], at.y != nullptr);
+                at.p.z = z[0], at.q.z = z[1];
+            }
             at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
-            kept = at.kept(true, table);
         }
-        if (tid < ranks) cluster_store(&keeps[round][rank], tid, (int)kept);  // to every CTA of the game
-        cluster_sync();
-        int first = ranks;
-        for (int k = ranks - 1; k >= 0; --k)
-            if (!keeps[round][k]) first = k;
-        if (kept && rank < first && tid == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
-        if (first == ranks) continue;
-        if (rank != first) return;
+        if (at.kept(true, table)) {  // the same for the whole game: all its CTAs have the same numbers
+            if (rank == 0 && tid == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
+            continue;
+        }
         int next = -1;
+        bool mine = rank == 0;  // whose share holds the point
         if (at.p.any && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
+            // the first of `count` whose running sum exceeds the point, or the last that has weight; `below`: the sum before it
+            auto find = [&](int count, auto &&weight, double &below, double target) {
+                double run = below, before = below;
+                int last = 0;
+                for (int k = 0; k < count; ++k) {
+                    const double w = weight(k);
+                    if (w > 0) {
+                        last = k, before = run;
+                        if (run + w > target) break;
+                    }
+                    run += w;
+                }
+                below = before;
+                return last;
+            };
+            // weights of [from, from + share), [from + share, ...): a warp's each
+            auto shares = [&](int from, int to, int share, bool residual) {
+                const int w0 = min(to, from + warp * share), w1 = min(to, w0 + share);
+                double part = 0;
+                if (residual && at.y) {
+#pragma unroll 4
+                    for (int j = w0 + lane; j < w1; j += 32) {
+                        const double pj = exp_neg((double)to_f(at.x[j]) - at.p.m, table) * at.p.iz;
+                        const double qj = exp_neg((double)to_f(at.y[j]) - at.q.m, table) * at.q.iz;
+                        part += fmax(pj - qj, 0.0);
+                    }
+                } else {
+#pragma unroll 4
+                    for (int j = w0 + lane; j < w1; j += 32) part += at.draw_weight(j, residual, table);
+                }
+                part = warp_sum(part);
+                __syncthreads();
+                if (lane == 0) sm.level[warp] = part;
+                __syncthreads();
+            };
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
                 const bool residual = pass == 0;
-                // the place of the point: an eighth of the row, of that an eighth, and so on, each warp a share
-                int from = 0, to = n;
-                double target = 0, below = 0;
-                bool none = false, wide = true;  // wide: the whole row, whose total is not known yet
-                while (to - from > 32) {
-                    const int share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
-                    const int w0 = min(to, from + warp * share), w1 = min(to, w0 + share);
-                    double part = 0;
-                    if (residual && at.y) {
-#pragma unroll 4
-                        for (int j = w0 + lane; j < w1; j += 32) {
-                            const double pj = exp_neg((double)to_f(at.x[j]) - at.p.m, table) * at.p.iz;
-                            const double qj = exp_neg((double)to_f(at.y[j]) - at.q.m, table) * at.q.iz;
-                            part += fmax(pj - qj, 0.0);
-                        }
-                    } else {
-#pragma unroll 4
-                        for (int j = w0 + lane; j < w1; j += 32) part += at.draw_weight(j, residual, table);
-                    }
-                    part = warp_sum(part);
-                    __syncthreads();
-                    if (lane == 0) level[warp] = part;
-                    __syncthreads();
-                    if (wide) {
-                        double total = 0;
-                        for (int k = 0; k < DENSE_WARPS; ++k) total += level[k];
-                        none = residual && !(total > RESIDUAL_MIN);
-                        target = r * total;
-                        wide = false;
-                    }
-                    if (none) break;
-                    // the first share whose running sum is above the point; with none, the last that has weight
-                    double run = below;
-                    int who = -1, last = 0;
-                    double at_last = below;
-                    for (int k = 0; k < DENSE_WARPS; ++k) {
-                        if (level[k] > 0) {
-                            last = k, at_last = run;
-                            if (run + level[k] > target) {
-                                who = k;
-                                break;
-                            }
-                        }
-                        run += level[k];
-                    }
-                    if (who < 0) who = last;
-                    below = at_last;
-                    const int f = min(to, from + who * share);
-                    to = min(to, f + share), from = f;
+                int from = s0, to = s1, share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
+                shares(from, to, share, residual);
+                double total = 0, below = 0;
+                for (int k = 0; k < DENSE_WARPS; ++k) total += sm.level[k];
+                if (ranks > 1) {
+                    if (tid == 0) tell(0, total);
+                    cluster_sync();
+                    total = 0;
+                    for (int k = 0; k < ranks; ++k) total += sm.told[round][k][0];
                 }
-                if (none) continue;
+                const double target = r * total;
+                if (residual && !(total > RESIDUAL_MIN)) {
+                    round ^= 1;
+                    continue;
+                }
+                if (ranks > 1) mine = find(ranks, [&](int k) { return sm.told[round][k][0]; }, below, target) == rank;
+                if (!mine) break;
+                // an eighth of the share, of that an eighth, and so on
+                for (;;) {
+                    const int who = find(DENSE_WARPS, [&](int k) { return sm.level[k]; }, below, target);
+                    from = min(to, from + who * share), to = min(to, from + share);
+                    if (to - from <= 32) break;
+                    share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
+                    shares(from, to, share, residual);
+                }
                 if (warp == 0) {
                     const int j = from + lane;
                     const double w = j < to ? at.draw_weight(j, residual, table) : 0.0;
                     const double above = warp_scan(w, lane);
-                    if (wide) {  // a row of at most 32 places
-                        const double total = __shfl_sync(ALL, above, 31);
-                        none = residual && !(total > RESIDUAL_MIN);
-                        target = r * total;
-                    }
                     const unsigned cross = __ballot_sync(ALL, w > 0 && below + above > target), some = __ballot_sync(ALL, w > 0);
-                    if (lane == 0) pick = none ? -2 : from + (cross ? __ffs(cross) - 1 : 31 - __clz(some));
+                    if (lane == 0) sm.pick = from + (cross ? __ffs(cross) - 1 : some ? 31 - __clz(some) : 0);
                 }
                 __syncthreads();
-                next = pick;
-                if (next == -2) {
-                    __syncthreads();
-                    continue;
-                }
+                next = sm.pick;
                 break;
             }
         }
+        if (!mine) return;
         if (tid == 0) {
             d.accepted[game] = i;
             out[i] = next;
@@ -761,25 +817,29 @@ __global__ void __launch_bounds__(DENSE_THREADS) verify_dense_kernel(const Verif
 template <typename T>
 static int verify_launch(const jq_drafts &d, cudaStream_t s) {
     VerifyArgs a{d, 1, 0};
-    const int places = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
     if (!d.mask) {
-        if ((int64_t)d.games * places > INT32_MAX) return fail(JQ_ERR_CAPACITY, "drafts: too many games for one call");
+        int sms, rc = device_sms(sms);
+        if (rc) return rc;
+        // enough CTAs for all SMs, several of which wait for one another's answers meanwhile, of a thousand places or more
+        int ctas = 1;
+        while (ctas < DENSE_CTAS && (int64_t)d.games * ctas < 6 * (int64_t)sms && d.actions > 1024 * ctas) ctas *= 2;
+        if ((int64_t)d.games * ctas > INT32_MAX) return fail(JQ_ERR_CAPACITY, "drafts: too many games for one call");
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)d.games * places);
+        cfg.gridDim = dim3((unsigned)d.games * ctas);
         cfg.blockDim = dim3(DENSE_THREADS);
         cfg.stream = s;
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = places, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr, cfg.numAttrs = 2;
         CU(cudaLaunchKernelEx(&cfg, verify_dense_kernel<T>, a));
         return JQ_OK;
     }
     a.share = 4 * (3 * LIST + (d.actions + 15 + 31) / 32 + 1);
     a.share = (a.share + 15) & ~15;
-    int warps = places;
+    int warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
     if (d.drafts == 0) warps = a.games_per_cta = 4;
     while (warps > 1 && (size_t)warps * a.share > 200 * 1024) --warps;
     if (d.drafts == 0) a.games_per_cta = warps;
