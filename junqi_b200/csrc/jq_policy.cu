@@ -31,59 +31,175 @@ __device__ __forceinline__ float ex2(float v) {
     return r;
 }
 
-// Bits of 32 mask bytes, byte 32 w first, from 16-byte loads of the aligned
-// blocks around them; at the row's ends, where those would leave the row,
-// byte by byte.
-__device__ __forceinline__ uint32_t legal_word(const uint8_t *row, int n, int w) {
-    const int j0 = 32 * w;
-    const uint8_t *p = row + j0;
-    const int a = (int)((uintptr_t)p & 15);
-    if (j0 >= a && (int64_t)j0 - a + (a ? 48 : 32) <= n) {
-        const uint4 *q = (const uint4 *)(p - a);
-        const uint4 u0 = q[0], u1 = q[1], u2 = a ? q[2] : make_uint4(0, 0, 0, 0);
-        uint32_t v[13] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w, u2.x, u2.y, u2.z, u2.w, 0};
-        const int s = a >> 2, f = (a & 3) * 8;
-        if (s & 2)
-#pragma unroll
-            for (int i = 0; i < 11; ++i) v[i] = v[i + 2];
-        if (s & 1)
-#pragma unroll
-            for (int i = 0; i < 10; ++i) v[i] = v[i + 1];
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __vminu4(__funnelshift_r(v[i], v[i + 1], f), 0x01010101u);
-            bits |= ((b * 0x01020408u) >> 24) << (4 * i);  // byte k's bit 8 k lands at 24 + k
-        }
-        return bits;
-    }
-    uint32_t bits = 0;
-    const int end = n - j0 < 32 ? n - j0 : 32;
-#pragma unroll 8
-    for (int i = 0; i < end; ++i) bits |= (uint32_t)(p[i] != 0) << i;
-    return bits;
+// Bits of 16 mask bytes, each 0 or 1: dot products with powers of two.
+__device__ __forceinline__ uint32_t pack_block(uint4 v) {
+    const uint32_t lo = __dp4a(v.y, 0x80402010u, __dp4a(v.x, 0x08040201u, 0u));
+    const uint32_t hi = __dp4a(v.w, 0x80402010u, __dp4a(v.z, 0x08040201u, 0u));
+    return lo + hi * 256;
 }
+__device__ __forceinline__ uint4 ones(uint4 v) {  // other truth values
+    return make_uint4(__vminu4(v.x, 0x01010101u), __vminu4(v.y, 0x01010101u), __vminu4(v.z, 0x01010101u), __vminu4(v.w, 0x01010101u));
+}
+
+// A row's mask in bits, in blocks of 16 bytes as they lie in memory: bit
+// (row & 15) + j for place j; by a warp, eight loads in flight a lane.  Blocks
+// with legal places go to `found` too, in order, as block << 16 | bits, as
+// long as there are at most `most`; their number is returned.
+__device__ __forceinline__ int pack_mask(uint16_t *bits, uint32_t *found, int most, const uint8_t *row, int places, int lane) {
+    constexpr int AHEAD = 8;
+    const int skip = (int)((uintptr_t)row & 15), blocks = (skip + places + 15) >> 4;
+    const uint8_t *first = row - skip;
+    const int k0 = skip ? 1 : 0, k1 = (skip + places) >> 4;  // whole blocks of the row
+    // the row's ends, a byte per lane, and the last word's upper half
+    const int ke = lane < 16 ? 0 : blocks - 1, je = 16 * ke + (lane & 15) - skip;
+    const bool end = lane < 16 ? k0 > 0 || k1 == 0 : k1 < blocks && blocks > 1;
+    const uint32_t ends = __ballot_sync(ALL, end && je >= 0 && je < places && row[je] != 0);
+    if ((lane & 15) == 0 && end) bits[ke] = (uint16_t)(lane ? ends >> 16 : ends);
+    if (lane == 0 && (blocks & 1)) bits[blocks] = 0;
+    int n = 0;
+    if (ends & 0xffff) {
+        if (lane == 0) found[0] = ends & 0xffff;
+        n = 1;
+    }
+    const uint32_t lower = (1u << lane) - 1;
+    for (int b0 = k0; b0 < k1; b0 += 32 * AHEAD) {
+        const uint8_t *from = first + 16 * (b0 + lane);
+        const int left = k1 - b0 - lane;
+        uint4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (32 * i < left) v[i] = *(const uint4 *)(from + 512 * i);
+        }
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) odd |= v[i].x | v[i].y | v[i].z | v[i].w;
+        if (__any_sync(ALL, odd & 0xfefefefeu))
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) v[i] = ones(v[i]);
+        uint16_t *to = bits + b0 + lane;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t b = pack_block(v[i]);
+            if (32 * i < left) to[32 * i] = (uint16_t)b;
+            const uint32_t some = __ballot_sync(ALL, b != 0);
+            const int at = n + __popc(some & lower);
+            if (b && at < most) found[at] = (uint32_t)(b0 + 32 * i + lane) << 16 | b;
+            n += __popc(some);
+        }
+    }
+    if (ends >> 16) {
+        if (lane == 0 && n < most) found[n] = (uint32_t)(blocks - 1) << 16 | ends >> 16;
+        ++n;
+    }
+    return n;
+}
+
+// A row's legal places, by a warp in its shared memory: the packed mask, and
+// the blocks of 16 that have some, as block << 16 | bits.  With more than LIST
+// blocks (or, for `list`, places) only the packed mask counts.  LIST is what
+// leaves room for 32 warps of verify_masked_kernel on an SM.
+constexpr int LIST = 320;
+struct Legal {
+    uint32_t *found, *bits;
+    int blocks, skip, words;
+    __device__ __forceinline__ Legal(char *at) : found((uint32_t *)at), bits((uint32_t *)at + LIST) {}
+    static size_t bytes(int places) { return (4 * (LIST + (places + 15 + 31) / 32 + 1) + 15) & ~(size_t)15; }
+    __device__ __forceinline__ void read(const uint8_t *mask, int places, int lane) {
+        skip = (int)((uintptr_t)mask & 15), words = (skip + places + 31) >> 5;
+        __syncwarp();  // the last row's has been read
+        blocks = pack_mask((uint16_t *)bits, found, LIST, mask, places, lane);
+        __syncwarp();
+    }
+    // The places in order, as far as there are at most LIST, and their number; [w0, w1): this lane's share of the words.
+    __device__ __forceinline__ int list(int *to, int lane, int &w0, int &w1) const {
+        const int share = (words + 31) >> 5;
+        w0 = min(words, lane * share), w1 = min(words, w0 + share);
+        // this lane's: of its share of the blocks that have some, or of the words
+        const bool few = blocks <= LIST;
+        const int per = (blocks + 31) >> 5, e0 = min(blocks, lane * per), e1 = min(blocks, e0 + per);
+        int before = 0;
+        if (few)
+            for (int e = e0; e < e1; ++e) before += __popc(found[e] & 0xffff);
+        else
+            for (int w = w0; w < w1; ++w) before += __popc(bits[w]);
+        const int own = before;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(ALL, before, o);
+            if (lane >= o) before += u;
+        }
+        const int count = __shfl_sync(ALL, before, 31);  // (more than LIST blocks have more than LIST places)
+        before -= own;
+        if (count <= LIST)
+            for (int e = e0; e < e1; ++e) {
+                const int j0 = (int)(found[e] >> 16) * 16 - skip;
+                for (uint32_t b = found[e] & 0xffff; b; b &= b - 1) to[before++] = j0 + __ffs(b) - 1;
+            }
+        __syncwarp();
+        return count;
+    }
+    __device__ __forceinline__ bool has(int j) const { return (bits[(j + skip) >> 5] >> ((j + skip) & 31)) & 1; }
+    // bits of places [32 w, 32 w + 32)
+    __device__ __forceinline__ uint32_t word(int w, int places) const {
+        const uint32_t hi = skip && w + 1 < words ? bits[w + 1] : 0, v = __funnelshift_r(bits[w], hi, skip);
+        return places - 32 * w >= 32 ? v : v & ((1u << (places - 32 * w)) - 1);
+    }
+};
+
+// The larger of two, or NaN where one is: so a maximum tells of every NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+constexpr float FAR = -3000.f;  // exp of it is 0, and so is its product with it: keeps -inf out of the sums
 
 // Running maximum, sum of exp(x - m) and sum of exp(x - m)(x - m).
 struct Soft {
     float m, s, t;
-    template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N]) {
-        float c = x[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) c = fmaxf(c, x[i]);
+    __device__ __forceinline__ void raise(float c) {
         if (c > m) {
             const float d = m - c, k = ex2(d * LOG2E);
             t = k > 0.f ? k * (t + s * d) : 0.f;  // k = 0: d may be far, or infinite
             s *= k;
             m = c;
         }
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N]) {
+        float c = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) c = fmaxf(c, x[i]);
+        raise(c);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float d = x[i] - m, e = ex2(d * LOG2E);
+            const float d = max_nan(x[i] - m, FAR), e = ex2(d * LOG2E);
             s += e;
-            if (e > 0.f) t += e * d;
+            t += e * d;
         }
+    }
+    template <int N>
+    __device__ __forceinline__ void add_pairs(const f2 (&x)[N]) {
+        float c = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c = fmaxf(c, fmaxf(parts(x[i]).x, parts(x[i]).y));
+        raise(c);
+        const f2 nm = both(-m), l = both(LOG2E);
+        f2 ss = both(0.f), tt = both(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float2 q = parts(x[i] + nm);
+            q.x = max_nan(q.x, FAR), q.y = max_nan(q.y, FAR);
+            const f2 d = make_f2(q.x, q.y);
+            const float2 w = parts(d * l);
+            const f2 e = make_f2(ex2(w.x), ex2(w.y));
+            ss = ss + e;
+            tt = fma2(e, d, tt);
+        }
+        s += parts(ss).x + parts(ss).y;
+        t += parts(tt).x + parts(tt).y;
     }
     __device__ __forceinline__ void join(float m2, float s2, float t2) {
         const float M = fmaxf(m, m2), d1 = m - M, d2 = m2 - M;
@@ -96,23 +212,6 @@ struct Soft {
     }
 };
 
-// A thread's legal logits, four loads in flight.
-template <typename T>
-__device__ __forceinline__ void add_bits(Soft &a, const T *x, uint32_t bits) {
-    while (bits) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = -INFINITY;
-            if (bits) {
-                v[i] = to_f(x[__ffs(bits) - 1]);
-                bits &= bits - 1;
-            }
-        }
-        a.add(v);
-    }
-}
-
 constexpr int LOGP_THREADS = 256;
 
 struct LogpArgs {
@@ -124,133 +223,188 @@ struct LogpArgs {
     float4 *stats;         // (rows): m, 1 / Z, log Z, H
     const float *glp, *gent;
     void *dx;
-    int64_t x_stride, mask_stride, glp_stride, gent_stride;
-    int32_t n, words;
+    int64_t rows, x_stride, mask_stride, glp_stride, gent_stride;
+    int32_t n, words, share;  // share: bytes of shared memory of a warp
 };
 
-__device__ __forceinline__ bool is_legal(const uint8_t *mask, const uint32_t *bits, int j) {
-    return bits ? (bits[j >> 5] >> (j & 31)) & 1 : !mask || mask[j] != 0;
+// A row's scores from its sums, by one thread.
+template <typename T>
+__device__ __forceinline__ void logp_finish(const LogpArgs &a, int64_t row, const Soft &acc, const T *x, int act, bool legal) {
+    const bool empty = acc.s == 0.f;
+    const float logz = empty ? 0.f : logf(acc.s), inv = empty ? 0.f : 1.f / acc.s;
+    const float h = empty ? 0.f : logz - acc.t * inv;
+    float lp = 0.f;
+    if (act >= 0 && act < a.n) {
+        // -inf at the action's place gives -inf, NaN anywhere legal NaN
+        lp = legal && !empty ? (to_f(x[act]) - acc.m) - logz : -INFINITY;
+        if (acc.s != acc.s) lp = acc.s;
+    }
+    a.lp[row] = lp;
+    a.ent[row] = h;
+    if (a.stats) a.stats[row] = make_float4(acc.m, inv, logz, h);
 }
 
-template <typename T, bool MASK>
-__global__ void __launch_bounds__(LOGP_THREADS) logp_fwd_kernel(const LogpArgs a) {
+__device__ __forceinline__ void warp_join(Soft &acc) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        acc.join(__shfl_xor_sync(ALL, acc.m, o), __shfl_xor_sync(ALL, acc.s, o), __shfl_xor_sync(ALL, acc.t, o));
+}
+
+// With a mask: a warp per row.
+constexpr int LOGP_WARPS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * LOGP_WARPS, 9) logp_masked_kernel(const LogpArgs a) {
+    extern __shared__ __align__(16) char logp_smem[];
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * LOGP_WARPS + warp;
+    if (row >= a.rows) return;
+    const T *x = (const T *)a.x + row * a.x_stride;
+    const int act = a.act[row];
+    Legal legal(logp_smem + warp * a.share);
+    legal.read(a.mask + row * a.mask_stride, a.n, lane);
+    Soft acc{LOWEST, 0.f, 0.f};
+    if (legal.blocks <= LIST) {
+        // a lane's blocks, four scattered logits in flight
+        uint32_t block = 0;
+        for (int e = lane; e < legal.blocks || (block & 0xffff);) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(block & 0xffff) && e < legal.blocks) block = legal.found[e], e += 32;
+                v[i] = -INFINITY;
+                if (block & 0xffff) {
+                    v[i] = to_f(x[(int)(block >> 16) * 16 - legal.skip + __ffs(block) - 1]);
+                    block &= block - 1;
+                }
+            }
+            acc.add(v);
+        }
+    } else {
+        for (int w = 0; w < legal.words; w += 8) {  // many: a lane per place, eight words at a time
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = 32 * (w + i) + lane - legal.skip;
+                v[i] = -INFINITY;
+                if (w + i < legal.words && (legal.bits[w + i] >> lane) & 1) v[i] = to_f(x[j]);
+            }
+            acc.add(v);
+        }
+    }
+    warp_join(acc);
+    if (lane == 0) logp_finish(a, row, acc, x, act, act >= 0 && act < a.n && legal.has(act));
+    if (a.bits)
+        for (int w = lane; w < a.words; w += 32) a.bits[row * a.words + w] = legal.word(w, a.n);
+}
+
+// Without: a CTA per row, 16 bytes a load, the ends one by one.
+template <typename T>
+__global__ void __launch_bounds__(LOGP_THREADS, 6) logp_dense_kernel(const LogpArgs a) {
+    constexpr int VEC = 16 / sizeof(T);
     __shared__ float red[LOGP_THREADS / 32][3];
     pdl_enter();
     const int64_t row = blockIdx.x;
     const T *x = (const T *)a.x + row * a.x_stride;
     const int tid = threadIdx.x, lane = tid & 31;
     Soft acc{LOWEST, 0.f, 0.f};
-    if (MASK) {
-        const uint8_t *mask = a.mask + row * a.mask_stride;
-        for (int w0 = tid - lane; w0 < a.words; w0 += LOGP_THREADS) {
-            const int w = w0 + lane;
-            const uint32_t bits = w < a.words ? legal_word(mask, a.n, w) : 0;
-            if (a.bits && w < a.words) a.bits[row * a.words + w] = bits;
-            // few legal places: each lane its own; many: the warp's words one after another, a lane per place
-            if (__reduce_add_sync(ALL, __popc(bits)) <= 256) {
-                add_bits(acc, x + 32 * w, bits);
-            } else {
-                for (int k = 0; k < 32; ++k) {
-                    const uint32_t b = __shfl_sync(ALL, bits, k);
-                    if (!b) continue;
-                    float v[1] = {(b >> lane) & 1 ? to_f(x[32 * (w0 + k) + lane]) : -INFINITY};
-                    acc.add(v);
-                }
+    const int head = min(a.n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+    const int packs = (a.n - head) / VEC;
+    const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
+    for (int k = tid; k < packs; k += 2 * LOGP_THREADS) {
+        Pack<T, VEC> p[2];
+        p[0] = px[k];
+        const bool two = k + LOGP_THREADS < packs;
+        if (two) p[1] = px[k + LOGP_THREADS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (h == 0 || two) {
+                f2 v[VEC / 2];
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i) v[i] = to_f2(&p[h].v[2 * i]);
+                acc.add_pairs(v);
             }
-        }
-    } else {
-        constexpr int VEC = 16 / sizeof(T);
-        const int head = min(a.n, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
-        const int packs = (a.n - head) / VEC;
-        const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
-        for (int k = tid; k < packs; k += LOGP_THREADS) {
-            const Pack<T, VEC> p = px[k];
-            float v[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = to_f(p.v[i]);
-            acc.add(v);
-        }
-        const int rest = a.n - packs * VEC;  // before the first pack and behind the last: at most 2 VEC - 2
-        if (tid < rest) {
-            float v[1] = {to_f(x[tid < head ? tid : tid + packs * VEC])};
-            acc.add(v);
-        }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        acc.join(__shfl_xor_sync(ALL, acc.m, o), __shfl_xor_sync(ALL, acc.s, o), __shfl_xor_sync(ALL, acc.t, o));
+    const int rest = a.n - packs * VEC;  // before the first pack and behind the last: at most 2 VEC - 2
+    if (tid < rest) {
+        float v[1] = {to_f(x[tid < head ? tid : tid + packs * VEC])};
+        acc.add(v);
+    }
+    warp_join(acc);
     if (lane == 0) red[tid >> 5][0] = acc.m, red[tid >> 5][1] = acc.s, red[tid >> 5][2] = acc.t;
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
         for (int i = 1; i < LOGP_THREADS / 32; ++i) acc.join(red[i][0], red[i][1], red[i][2]);
-        const bool empty = acc.s == 0.f;
-        const float logz = empty ? 0.f : logf(acc.s), inv = empty ? 0.f : 1.f / acc.s;
-        const float h = empty ? 0.f : logz - acc.t * inv;
-        const int act = a.act[row];
-        float lp = 0.f;
-        if (act >= 0 && act < a.n) {
-            const bool legal = !MASK || a.mask[row * a.mask_stride + act] != 0;
-            // -inf at the action's place gives -inf, NaN anywhere legal NaN
-            lp = legal && !empty ? (to_f(x[act]) - acc.m) - logz : -INFINITY;
-            if (acc.s != acc.s) lp = acc.s;
-        }
-        a.lp[row] = lp;
-        a.ent[row] = h;
-        if (a.stats) a.stats[row] = make_float4(acc.m, inv, logz, h);
+        logp_finish(a, row, acc, x, a.act[row], true);
     }
 }
 
-// Gradient: zeros over the row, then the legal places.
+// Gradient.  With a mask: zeros over the row, then the legal places; what they
+// need is fetched before the zeros are written, so that it arrives meanwhile.
 template <typename T, bool MASK>
 __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a) {
-    constexpr int VEC = 16 / sizeof(T);
+    constexpr int VEC = 16 / sizeof(T), AHEAD = 4;
     pdl_enter();
     const int64_t row = blockIdx.x;
     const T *x = (const T *)a.x + row * a.x_stride;
     T *dx = (T *)a.dx + row * a.n;
     const int tid = threadIdx.x, lane = tid & 31;
+    const uint32_t *bits = MASK ? a.bits + row * a.words : nullptr;
+    uint32_t mine = MASK && tid < a.words ? bits[tid] : 0, more = MASK && tid + LOGP_THREADS < a.words ? bits[tid + LOGP_THREADS] : 0;
     const float4 st = a.stats[row];  // m, 1 / Z, log Z, H
     const int act = a.act[row];
-    const uint32_t *bits = MASK ? a.bits + row * a.words : nullptr;
-    // the action's gradient: none without an action, or with one whose log-probability is -inf
-    const bool taken = act >= 0 && act < a.n && (!MASK || is_legal(nullptr, bits, act)) && to_f(x[act]) != -INFINITY;
-    const float u = taken && a.glp ? a.glp[row * a.glp_stride] : 0.f;
+    const bool inside = act >= 0 && act < a.n;
+    const bool legal = inside && (!MASK || ((bits[act >> 5] >> (act & 31)) & 1));
+    const float xa = inside ? to_f(x[act]) : 0.f;
+    float u = a.glp ? a.glp[row * a.glp_stride] : 0.f;
     const float v = a.gent ? a.gent[row * a.gent_stride] : 0.f;
+    // -p (u + v (log p + H)) = exp(c) (k0 + k1 c)
+    float k0 = 0.f, k1 = -v * st.y;
     auto grad = [&](int j, float xj) {
-        const float c = xj - st.x, p = ex2(c * LOG2E) * st.y;
-        const float g = -p * (u + v * (c - st.z + st.w));
-        return (p == 0.f ? 0.f : g) + (j == act ? u : 0.f);
+        const float c = max_nan(xj - st.x, FAR);
+        return ex2(c * LOG2E) * fmaf(k1, c, k0) + (j == act ? u : 0.f);
     };
     const int head = min(a.n, (int)((16 - ((uintptr_t)dx & 15)) & 15) / (int)sizeof(T));
     const int packs = (a.n - head) / VEC, rest = a.n - packs * VEC;
     Pack<T, VEC> *pd = (Pack<T, VEC> *)(dx + head);
     if (MASK) {
+        // the first few legal places of this thread's first two words
+        float xs[AHEAD];
+        int at[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            at[i] = -1;
+            if (mine) {
+                at[i] = 32 * tid + __ffs(mine) - 1;
+                mine &= mine - 1;
+            } else if (more) {
+                at[i] = 32 * (tid + LOGP_THREADS) + __ffs(more) - 1;
+                more &= more - 1;
+            }
+            if (at[i] >= 0) xs[i] = to_f(x[at[i]]);
+        }
         Pack<T, VEC> zero;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) zero.v[i] = from_f<T>(0.f);
         for (int k = tid; k < packs; k += LOGP_THREADS) pd[k] = zero;
         if (tid < rest) dx[tid < head ? tid : tid + packs * VEC] = zero.v[0];
+        // the action's gradient: none without an action, or with one whose log-probability is -inf
+        if (!legal || xa == -INFINITY) u = 0.f;
+        k0 = -(u + v * (st.w - st.z)) * st.y;
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (at[i] >= 0) dx[at[i]] = from_f<T>(grad(at[i], xs[i]));
         for (int w0 = tid - lane; w0 < a.words; w0 += LOGP_THREADS) {
             const int w = w0 + lane;
-            uint32_t b = w < a.words ? bits[w] : 0;
-            if (__reduce_add_sync(ALL, __popc(b)) <= 256) {
-                while (b) {
-                    float g[4];
-                    int at[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        at[i] = -1;
-                        if (b) {
-                            at[i] = 32 * w + __ffs(b) - 1;
-                            b &= b - 1;
-                            g[i] = to_f(x[at[i]]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (at[i] >= 0) dx[at[i]] = from_f<T>(grad(at[i], g[i]));
+            uint32_t b = w == tid ? mine : w == tid + LOGP_THREADS ? more : w < a.words ? bits[w] : 0;
+            // few legal places: each lane its own; many: the warp's words one after another, a lane per place
+            if (__reduce_add_sync(ALL, __popc(b)) <= 128) {
+                for (; b; b &= b - 1) {
+                    const int j = 32 * w + __ffs(b) - 1;
+                    dx[j] = from_f<T>(grad(j, to_f(x[j])));
                 }
             } else {
                 for (int k = 0; k < 32; ++k) {
@@ -261,8 +415,12 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
             }
         }
     } else {
+        if (!legal || xa == -INFINITY) u = 0.f;
+        k0 = -(u + v * (st.w - st.z)) * st.y;
         const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;  // x's packs start where dx's do
         const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
+        const f2 nm = both(-st.x), l = both(LOG2E), f0 = both(k0), f1 = both(k1);
+#pragma unroll 2
         for (int k = tid; k < packs; k += LOGP_THREADS) {
             const int j = head + k * VEC;
             Pack<T, VEC> p;
@@ -271,8 +429,21 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
             else
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) p.v[i] = x[j + i];
+            f2 g[VEC / 2];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) p.v[i] = from_f<T>(grad(j + i, to_f(p.v[i])));
+            for (int i = 0; i < VEC / 2; ++i) {
+                float2 q = parts(to_f2(&p.v[2 * i]) + nm);
+                q.x = max_nan(q.x, FAR), q.y = max_nan(q.y, FAR);
+                const f2 c = make_f2(q.x, q.y);
+                const float2 w = parts(c * l);
+                g[i] = make_f2(ex2(w.x), ex2(w.y)) * fma2(c, f1, f0);
+            }
+            if ((unsigned)(act - j) < (unsigned)VEC)  // the action's pack
+#pragma unroll
+                for (int i = 0; i < VEC / 2; ++i)
+                    g[i] = g[i] + make_f2(j + 2 * i == act ? u : 0.f, j + 2 * i + 1 == act ? u : 0.f);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) from_f2(&p.v[2 * i], g[i]);
             pd[k] = p;
         }
         if (tid < rest) {
@@ -305,7 +476,6 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
 constexpr int PLACES = 8;      // of a game at the same time
-constexpr int LIST = 320;      // legal actions of a place's list; with more, the packed mask is walked instead
 
 struct VerifyArgs {
     jq_drafts d;
@@ -321,32 +491,37 @@ struct VerifyArgs {
 // banks of their own.
 constexpr int EXP_STEPS = 16;
 __device__ __forceinline__ double exp_table(int i) { return exp2((double)i / EXP_STEPS); }
-__device__ __forceinline__ double exp_neg(double d, const double *table) {
+// 16 / ln 2, -ln 2 / 16, 1 / 5!, 1 / 4!, 1 / 3!: as constants in memory they are operands; written into the code,
+// each use takes two more instructions to make one
+__constant__ double c_exp[5] = {EXP_STEPS * 1.4426950408889634, -0.69314718055994531 / EXP_STEPS, 1.0 / 120, 1.0 / 24, 1.0 / 6};
+__device__ __forceinline__ double exp_near(double d, const double *table) {  // d in [-700, 0]
+    static_assert(EXP_STEPS == 16, "four bits of k are the table's");
     constexpr double MAGIC = 1.5 * 4503599627370496.0;  // 1.5 * 2^52: a sum's last bit is 1
-    constexpr double PER = EXP_STEPS * 1.4426950408889634, LN = 0.69314718055994531 / EXP_STEPS;
-    const double near = fma(d, PER, MAGIC);
+    const double near = fma(d, c_exp[0], MAGIC);
     const int k = __double2loint(near);
-    const double r = fma(near - MAGIC, -LN, d);
-    const double e = r * fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0);
-    const double at = table[k & (EXP_STEPS - 1)];
-    const double v = fma(at, e, at);
-    static_assert(EXP_STEPS == 16, "k >> 4");
-    const double scaled = __hiloint2double(__double2hiint(v) + ((k >> 4) << 20), __double2loint(v));
-    return d < -700.0 ? 0.0 : d == d ? scaled : d;
+    const double r = fma(near - MAGIC, c_exp[1], d);
+    const double e = r * fma(r, fma(r, fma(r, fma(r, c_exp[2], c_exp[3]), c_exp[4]), 0.5), 1.0);
+    const double at = table[k & 15], v = fma(at, e, at);
+    return __hiloint2double(__double2hiint(v) + ((k & ~15) << 16), __double2loint(v));
 }
 
 // One row of logits and what its probabilities need.
 struct Dist {
     double m, z, iz; // the largest logit, Z and its reciprocal
+    float low;       // logits below it have exp(x - m) = 0
     bool any;        // a legal place above -inf
-    __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)
-        return any ? exp_neg((double)x - m, table) : x != x ? (double)x : 0.0;
-    }
+    bool broken;     // NaN or +inf at a legal place: no distribution
     __device__ __forceinline__ void start(float top, bool there) {
-        any = there && top > -INFINITY;
-        m = top, z = iz = 0;
+        broken = there && !(top < INFINITY);
+        any = there && !broken && top > -INFINITY;
+        m = any ? top : 0.f;
+        low = any ? (float)(m - 700.0) : INFINITY;  // (rounded to m itself where m is beyond 2^33: the next logit is far)
+        z = iz = 0;
     }
-    __device__ __forceinline__ bool broken() const { return z != z; }  // NaN or +inf at a legal place
+    __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)
+        const double e = exp_near((double)x - m, table);
+        return x >= low ? e : 0.0;
+    }
 };
 
 // What a place is, and whether its draft is kept.
@@ -356,11 +531,11 @@ struct Place {
     const uint8_t *mask;
     int act;              // the drafted action; -1 behind the last
     bool drafted;         // i < len
-    float u;
+    float u, xa, ya;      // the draft's random number, the drafted action's logits
     Dist p, q;
     __device__ __forceinline__ Place(const jq_drafts &d, int game, int i, int len)
         : x((const T *)d.logits + game * d.logits_game + i * d.logits_place), y(nullptr),
-          mask(d.mask ? d.mask + game * d.mask_game + i * d.mask_place : nullptr), act(-1), drafted(i < len), u(0.f) {
+          mask(d.mask ? d.mask + game * d.mask_game + i * d.mask_place : nullptr), act(-1), drafted(i < len), u(0.f), xa(0.f), ya(0.f) {
         if (drafted) {
             act = d.drafted[(int64_t)game * d.drafts + i];
             u = d.accept_u[(int64_t)game * d.drafts + i];
@@ -368,11 +543,17 @@ struct Place {
         }
         if (act >= d.actions) act = -1;
     }
-    __device__ __forceinline__ bool broken() const { return p.broken() || q.broken(); }
+    __device__ __forceinline__ void fetch() {  // the drafted action's logits, some time after the action itself
+        if (act >= 0) {
+            xa = to_f(x[act]);
+            if (y) ya = to_f(y[act]);
+        }
+    }
+    __device__ __forceinline__ bool broken() const { return p.broken || q.broken; }
     __device__ __forceinline__ bool kept(bool legal, const double *table) const {
         if (act < 0 || !legal || broken() || !p.any) return false;
-        const double pa = p.weight(to_f(x[act]), table) * p.iz;
-        const double qa = !y ? 1.0 : q.any ? q.weight(to_f(y[act]), table) * q.iz : 0.0;
+        const double pa = p.weight(xa, table) * p.iz;
+        const double qa = !y ? 1.0 : q.any ? q.weight(ya, table) * q.iz : 0.0;
         return (double)u * qa < pa;
     }
     // the distribution that is drawn from: max(p - q, 0) while `residual`, else p
@@ -398,7 +579,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(ALL, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(ALL, v, o));
     return v;
 }
 __device__ __forceinline__ double warp_scan(double v, int lane) {
@@ -408,63 +589,6 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
         if (lane >= o) v += u;
     }
     return v;
-}
-
-// Bits of 16 mask bytes: bytes of 0 and 1 are dot products with powers of two.
-__device__ __forceinline__ uint32_t pack_block(uint4 v) {
-    if ((v.x | v.y | v.z | v.w) & 0xfefefefeu)  // other truth values
-        v = make_uint4(__vminu4(v.x, 0x01010101u), __vminu4(v.y, 0x01010101u), __vminu4(v.z, 0x01010101u), __vminu4(v.w, 0x01010101u));
-    const uint32_t lo = __dp4a(v.y, 0x80402010u, __dp4a(v.x, 0x08040201u, 0u));
-    const uint32_t hi = __dp4a(v.w, 0x80402010u, __dp4a(v.z, 0x08040201u, 0u));
-    return lo | hi << 8;
-}
-
-// A row's mask in bits, in blocks of 16 bytes as they lie in memory: bit
-// (row & 15) + j for place j; by a warp, eight loads in flight a lane.  Blocks
-// with legal places go to `found` too, in order, as block << 16 | bits, as
-// long as there are at most `most`; their number is returned.
-__device__ __forceinline__ int pack_mask(uint16_t *bits, uint32_t *found, int most, const uint8_t *row, int places, int lane) {
-    constexpr int AHEAD = 8;
-    const int skip = (int)((uintptr_t)row & 15), blocks = (skip + places + 15) >> 4;
-    const uint8_t *first = row - skip;
-    const int k0 = skip ? 1 : 0, k1 = (skip + places) >> 4;  // whole blocks of the row
-    // the row's ends, a byte per lane, and the last word's upper half
-    const int ke = lane < 16 ? 0 : blocks - 1, je = 16 * ke + (lane & 15) - skip;
-    const bool end = lane < 16 ? k0 > 0 || k1 == 0 : k1 < blocks && blocks > 1;
-    const uint32_t ends = __ballot_sync(ALL, end && je >= 0 && je < places && row[je] != 0);
-    if ((lane & 15) == 0 && end) bits[ke] = (uint16_t)(lane ? ends >> 16 : ends);
-    if (lane == 0 && (blocks & 1)) bits[blocks] = 0;
-    int n = 0;
-    if (ends & 0xffff) {
-        if (lane == 0) found[0] = ends & 0xffff;
-        n = 1;
-    }
-    for (int b0 = k0; b0 < k1; b0 += 32 * AHEAD) {
-        uint4 v[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int k = b0 + 32 * i + lane;
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (k < k1) v[i] = *(const uint4 *)(first + 16 * k);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int k = b0 + 32 * i + lane;
-            const uint32_t b = pack_block(v[i]);
-            if (k < k1) bits[k] = (uint16_t)b;
-            const uint32_t some = __ballot_sync(ALL, b != 0);
-            if (b) {
-                const int at = n + __popc(some & ((1u << lane) - 1));
-                if (at < most) found[at] = (uint32_t)k << 16 | b;
-            }
-            n += __popc(some);
-        }
-    }
-    if (ends >> 16) {
-        if (lane == 0 && n < most) found[n] = (uint32_t)(blocks - 1) << 16 | ends >> 16;
-        ++n;
-    }
-    return n;
 }
 
 template <typename T>
@@ -477,9 +601,10 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
     for (int i = threadIdx.x; i < EXP_STEPS; i += blockDim.x) table[i] = exp_table(i);
     pdl_enter();
     __syncthreads();
-    int *list = (int *)(verify_smem + warp * a.share);     // the legal actions in order, their logits, the draft's
-    float *lx = (float *)(list + LIST), *ly = lx + LIST;
-    uint32_t *bits = (uint32_t *)(ly + LIST);
+    Legal legal(verify_smem + warp * a.share);
+    // the legal actions in order and their logits (in what was scratch); the draft's, which there is room for if there are any
+    int *list = (int *)(verify_smem + (warp + 1) * a.share) - LIST;
+    float *lx = (float *)legal.found, *ly = (float *)(list - LIST);
     const bool alone = a.games_per_cta > 1;  // a game is this warp's, and has one place
     const int game = alone ? blockIdx.x * a.games_per_cta + warp : blockIdx.x;
     if (game >= d.games) return;             // (alone: no barrier follows)
@@ -492,50 +617,26 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
         const bool active = i <= len;
         bool kept = false;
         Place<T> at(d, game, active ? i : len, len);
-        int count = 0, lo = 0, hi = 0;
-        const int skip = (int)((uintptr_t)at.mask & 15), words = (skip + n + 31) >> 5;
-        const int share = (words + 31) >> 5, w0 = min(words, lane * share), w1 = min(words, w0 + share);
+        int count = 0, lo = 0, hi = 0, w0 = 0, w1 = 0;
         // this lane's legal actions, consecutive ones, with their logits: of the list, or of the packed mask
         auto each = [&](auto &&f) {
             if (count <= LIST) {
-                for (int k = lo; k < hi; ++k) f(list[k], lx[k], ly[k]);
+                for (int k = lo; k < hi; ++k) f(list[k], lx[k], at.y ? ly[k] : 0.f);
             } else {
                 for (int w = w0; w < w1; ++w)
-                    for (uint32_t b = bits[w]; b; b &= b - 1) {
-                        const int j = 32 * w + __ffs(b) - 1 - skip;
+                    for (uint32_t b = legal.bits[w]; b; b &= b - 1) {
+                        const int j = 32 * w + __ffs(b) - 1 - legal.skip;
                         f(j, to_f(at.x[j]), at.y ? to_f(at.y[j]) : 0.f);
                     }
             }
         };
         if (active) {
-            __syncwarp();
-            uint32_t *found = (uint32_t *)lx;
-            const int blocks = pack_mask((uint16_t *)bits, found, LIST, at.mask, n, lane);
-            __syncwarp();
-            // this lane's legal places: of its share of the blocks that have some, or of the words
-            const bool few = blocks <= LIST;
-            const int per_lane = (blocks + 31) >> 5, e0 = min(blocks, lane * per_lane), e1 = min(blocks, e0 + per_lane);
-            int before = 0;
-            if (few)
-                for (int e = e0; e < e1; ++e) before += __popc(found[e] & 0xffff);
-            else
-                for (int w = w0; w < w1; ++w) before += __popc(bits[w]);
-            const int own = before;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(ALL, before, o);
-                if (lane >= o) before += u;
-            }
-            count = __shfl_sync(ALL, before, 31);
-            before -= own;
+            legal.read(at.mask, n, lane);
+            at.fetch();
+            count = legal.list(list, lane, w0, w1);
             if (count <= LIST) {
-                for (int e = e0; e < e1; ++e) {
-                    const int j0 = (int)(found[e] >> 16) * 16 - skip;
-                    for (uint32_t b = found[e] & 0xffff; b; b &= b - 1) list[before++] = j0 + __ffs(b) - 1;
-                }
                 const int per = (count + 31) >> 5;
                 lo = min(count, lane * per), hi = min(count, lo + per);
-                __syncwarp();
                 for (int k0 = 0; k0 < count; k0 += 128) {  // four scattered logits of each in flight
                     float vx[4], vy[4];
 #pragma unroll
@@ -549,13 +650,14 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int k = k0 + 32 * i + lane;
-                        if (k < count) lx[k] = vx[i], ly[k] = at.y ? vy[i] : 0.f;
+                        if (k < count) lx[k] = vx[i];
+                        if (k < count && at.y) ly[k] = vy[i];
                     }
                 }
                 __syncwarp();
             }
             float mx = -INFINITY, my = -INFINITY;
-            each([&](int, float x, float y) { mx = fmaxf(mx, x), my = fmaxf(my, y); });
+            each([&](int, float x, float y) { mx = max_nan(mx, x), my = max_nan(my, y); });
             at.p.start(warp_max(mx), true);
             at.q.start(warp_max(my), at.y != nullptr);
             double zx = 0, zy = 0;
@@ -565,8 +667,7 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
             });
             at.p.z = warp_sum(zx), at.q.z = warp_sum(zy);
             at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
-            const int b = at.act + skip;
-            kept = at.kept(at.act >= 0 && ((bits[b >> 5] >> (b & 31)) & 1), table);
+            kept = at.kept(at.act >= 0 && legal.has(at.act), table);
         }
         int first = alone ? 0 : warps;  // the first place of this round that is not kept
         if (!alone) {
@@ -615,203 +716,213 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
     }
 }
 
-// Without a mask: a cluster per game, each CTA a consecutive share of every
-// row.  Place by place, since a place is enough work for the whole cluster:
-// no row behind the first rejection is read.
+// Without a mask: a cluster of CTAs per game, each warp a consecutive chunk of
+// every row.  Place by place, since a place is enough work for the whole
+// cluster: no row behind the first rejection is read (the next one is fetched
+// into L2 meanwhile).  A warp takes its own maximum and sum, and all tell all
+// others once per place and once for the draw; then the warp that has the
+// point goes on alone.
 constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32, DENSE_CTAS = 8;
 
-// Every logit of x[0, n), by the CTA: 8 bytes a load, the ends one by one.
+// Every logit of x[0, n), by the warp: 8 bytes a load, the ends one by one.
 template <typename T, typename F>
-__device__ __forceinline__ void dense_each(const T *x, int n, int tid, F &&f) {
+__device__ __forceinline__ void dense_each(const T *x, int n, int lane, F &&f) {
     constexpr int VEC = 8 / sizeof(T);
     const int head = min(n, (int)((8 - ((uintptr_t)x & 7)) & 7) / (int)sizeof(T)), packs = (n - head) / VEC;
     const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
-    int k = tid;
-    for (; k + 3 * DENSE_THREADS < packs; k += 4 * DENSE_THREADS) {
+    int k = lane;
+    for (; k + 96 < packs; k += 128) {
         Pack<T, VEC> p[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) p[u] = px[k + u * DENSE_THREADS];
+        for (int u = 0; u < 4; ++u) p[u] = px[k + 32 * u];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) f(to_f(p[u].v[i]));
     }
-    for (; k < packs; k += DENSE_THREADS) {
+    for (; k < packs; k += 32) {
         const Pack<T, VEC> p = px[k];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) f(to_f(p.v[i]));
     }
     const int rest = n - packs * VEC;  // before the first pack and behind the last
-    if (tid < rest) f(to_f(x[tid < head ? tid : tid + packs * VEC]));
+    if (lane < rest) f(to_f(x[lane < head ? lane : lane + packs * VEC]));
 }
 
-// Sum of exp(x - m) over this thread's logits of x[0, n).
+// The largest of x[0, n), and the sum of exp(x - it), of a warp's chunk.
 template <typename T>
-__device__ __forceinline__ double dense_sum(const T *x, int n, int tid, const Dist &d, const double *table) {
+__device__ __forceinline__ float dense_top(const T *x, int n, int lane) {
+    float top = -INFINITY;
+    dense_each(x, n, lane, [&](float v) { top = max_nan(top, v); });
+    return top;
+}
+template <typename T>
+__device__ __forceinline__ double dense_sum(const T *x, int n, int lane, const Dist &d, const double *table) {
     double z = 0;
-    if (d.any)
-        dense_each(x, n, tid, [&](float v) { z += exp_neg((double)v - d.m, table); });
-    else
-        dense_each(x, n, tid, [&](float v) { z += v != v ? (double)v : 0.0; });
+    if (d.any) dense_each(x, n, lane, [&](float v) { z += d.weight(v, table); });
     return z;
 }
 
-struct DenseSmem {
-    double table[EXP_STEPS];
-    double sums[2][DENSE_WARPS], level[DENSE_WARPS];
-    float tops[2][DENSE_WARPS];
-    double told[2][DENSE_CTAS][4];  // what the game's CTAs tell each other: two rounds' m, Z of the target, m, Z of the draft
-    int pick;
-};
-
 template <typename T>
 __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const VerifyArgs a) {
-    __shared__ DenseSmem sm;
+    __shared__ double table[EXP_STEPS];
+    __shared__ double told[2][DENSE_CTAS * DENSE_WARPS][4];  // by every warp of the game: m, Z of the target, m, Z of the draft
     const jq_drafts &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = d.actions;
+    const int tid = threadIdx.x, lane = tid & 31, n = d.actions;
     const int rank = (int)cluster_rank(), ranks = (int)cluster_size(), game = blockIdx.x / ranks;
-    if (tid < EXP_STEPS) sm.table[tid] = exp_table(tid);
-    const double *table = sm.table;
+    const int warps = ranks * DENSE_WARPS, me = rank * DENSE_WARPS + (tid >> 5);
+    if (tid < EXP_STEPS) table[tid] = exp_table(tid);
     pdl_enter();
     cluster_sync();  // the game's CTAs have all started: their shared memory may be written
     int len = d.lengths ? d.lengths[game] : d.drafts;
     len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
     int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
     float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
-    const int all = ((n + ranks - 1) / ranks + 31) & ~31, s0 = min(n, rank * all), s1 = min(n, s0 + all);
+    const int chunk = (n + warps - 1) / warps, c0 = min(n, me * chunk), c1 = min(n, c0 + chunk);
     int round = 0;
-    // `v` (of thread 0) of every CTA to every CTA, as told[round][rank][at]
-    auto tell = [&](int at, double v) {
-        for (int k = 0; k < ranks; ++k) cluster_store(&sm.told[round][rank][at], k, v);
+    // four numbers of this warp to every CTA
+    auto tell = [&](double v0, double v1, double v2, double v3) {
+        const int what = lane & 3;
+        if (lane < 4 * ranks) cluster_store(&told[round][me][what], lane >> 2, what == 0 ? v0 : what == 1 ? v1 : what == 2 ? v2 : v3);
+        cluster_sync();
     };
     for (int i = 0;; ++i) {
         Place<T> at(d, game, i, len);
         {
-            float mx = -INFINITY, my = -INFINITY;
-            dense_each(at.x + s0, s1 - s0, tid, [&](float v) { mx = fmaxf(mx, v); });
-            if (at.y) dense_each(at.y + s0, s1 - s0, tid, [&](float v) { my = fmaxf(my, v); });
-            mx = warp_max(mx), my = warp_max(my);
-            __syncthreads();
-            if (lane == 0) sm.tops[0][warp] = mx, sm.tops[1][warp] = my;
-            __syncthreads();
-            for (int k = 0; k < DENSE_WARPS; ++k) mx = fmaxf(mx, sm.tops[0][k]), my = fmaxf(my, sm.tops[1][k]);
-            at.p.start(mx, true), at.q.start(my, at.y != nullptr);
-            double zx = dense_sum(at.x + s0, s1 - s0, tid, at.p, table);
-            double zy = at.y ? dense_sum(at.y + s0, s1 - s0, tid, at.q, table) : 0.0;
-            zx = warp_sum(zx), zy = warp_sum(zy);
-            if (lane == 0) sm.sums[0][warp] = zx, sm.sums[1][warp] = zy;
-            __syncthreads();
-            for (int k = 0; k < DENSE_WARPS; ++k) at.p.z += sm.sums[0][k], at.q.z += sm.sums[1][k];
-            if (ranks > 1) {
-                if (tid == 0) tell(0, at.p.m), tell(1, at.p.z), tell(2, at.q.m), tell(3, at.q.z);
-                cluster_sync();
-                double m[2] = {-INFINITY, -INFINITY}, z[2] = {0, 0};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    for (int k = 0; k < ranks; ++k) m[h] = fmax(m[h], sm.told[round][k][2 * h]);
-                    for (int k = 0; k < ranks; ++k) {
-                        const double mk = sm.told[round][k][2 * h], zk = sm.told[round][k][2 * h + 1];
-                        z[h] += mk > -INFINITY ? zk * exp_neg(mk - m[h], table) : zk;  // (a share of -inf has Z = 0 or NaN)
-                    }
-                }
-                round ^= 1;
-                at.p.start((float)m[0], true), at.q.start((float)m[1], at.y != nullptr);
-                at.p.z = z[0], at.q.z = z[1];
+            float mx, my = -INFINITY;
+            double zx, zy = 0;
+            Dist own;
+            if (i < len && 64 * lane < (c1 - c0) * (int)sizeof(T)) {  // the next place's chunk, on its way into L2
+                const int64_t by = (int64_t)c0 + 64 / (int)sizeof(T) * lane;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at.x + d.logits_place + by));
+                if (i + 1 < len && at.y) asm volatile("prefetch.global.L2 [%0];" ::"l"(at.y + d.draft_place + by));
             }
-            at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
+            mx = dense_top(at.x + c0, c1 - c0, lane);
+            if (at.y) my = dense_top(at.y + c0, c1 - c0, lane);
+            at.fetch();
+            mx = warp_max(mx), my = warp_max(my);
+            own.start(mx, true);
+            zx = dense_sum(at.x + c0, c1 - c0, lane, own, table);
+            if (at.y) {
+                own.start(my, true);
+                zy = dense_sum(at.y + c0, c1 - c0, lane, own, table);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) zx += __shfl_xor_sync(ALL, zx, o), zy += __shfl_xor_sync(ALL, zy, o);
+            tell((double)mx, zx, (double)my, zy);
+            const int k1 = lane + 32;
+            const float m0 = lane < warps ? (float)told[round][lane][0] : -INFINITY, m1 = k1 < warps ? (float)told[round][k1][0] : -INFINITY;
+            const float q0 = lane < warps ? (float)told[round][lane][2] : -INFINITY, q1 = k1 < warps ? (float)told[round][k1][2] : -INFINITY;
+            at.p.start(warp_max(max_nan(m0, m1)), true);
+            at.q.start(warp_max(max_nan(q0, q1)), at.y != nullptr);
+            double z = lane < warps ? told[round][lane][1] * at.p.weight(m0, table) : 0.0;
+            if (k1 < warps) z += told[round][k1][1] * at.p.weight(m1, table);
+            at.p.z = warp_sum(z), at.p.iz = 1.0 / at.p.z;
+            if (at.y) {
+                z = lane < warps ? told[round][lane][3] * at.q.weight(q0, table) : 0.0;
+                if (k1 < warps) z += told[round][k1][3] * at.q.weight(q1, table);
+                at.q.z = warp_sum(z), at.q.iz = 1.0 / at.q.z;
+            }
+            round ^= 1;
         }
-        if (at.kept(true, table)) {  // the same for the whole game: all its CTAs have the same numbers
-            if (rank == 0 && tid == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
+        if (at.kept(true, table)) {  // the same for the whole game: all its warps have the same numbers
+            if (me == 0 && lane == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
             continue;
         }
-        int next = -1;
-        bool mine = rank == 0;  // whose share holds the point
+        int next = -1, who = 0;  // who: the warp whose chunk has the point
         if (at.p.any && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
-            // the first of `count` whose running sum exceeds the point, or the last that has weight; `below`: the sum before it
-            auto find = [&](int count, auto &&weight, double &below, double target) {
-                double run = below, before = below;
-                int last = 0;
-                for (int k = 0; k < count; ++k) {
-                    const double w = weight(k);
-                    if (w > 0) {
-                        last = k, before = run;
-                        if (run + w > target) break;
-                    }
-                    run += w;
-                }
-                below = before;
-                return last;
-            };
-            // weights of [from, from + share), [from + share, ...): a warp's each
-            auto shares = [&](int from, int to, int share, bool residual) {
-                const int w0 = min(to, from + warp * share), w1 = min(to, w0 + share);
-                double part = 0;
-                if (residual && at.y) {
-#pragma unroll 4
-                    for (int j = w0 + lane; j < w1; j += 32) {
-                        const double pj = exp_neg((double)to_f(at.x[j]) - at.p.m, table) * at.p.iz;
-                        const double qj = exp_neg((double)to_f(at.y[j]) - at.q.m, table) * at.q.iz;
-                        part += fmax(pj - qj, 0.0);
-                    }
-                } else {
-#pragma unroll 4
-                    for (int j = w0 + lane; j < w1; j += 32) part += at.draw_weight(j, residual, table);
-                }
-                part = warp_sum(part);
-                __syncthreads();
-                if (lane == 0) sm.level[warp] = part;
-                __syncthreads();
-            };
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
-                const bool residual = pass == 0;
-                int from = s0, to = s1, share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
-                shares(from, to, share, residual);
-                double total = 0, below = 0;
-                for (int k = 0; k < DENSE_WARPS; ++k) total += sm.level[k];
-                if (ranks > 1) {
-                    if (tid == 0) tell(0, total);
-                    cluster_sync();
-                    total = 0;
-                    for (int k = 0; k < ranks; ++k) total += sm.told[round][k][0];
+                const bool residual = pass == 0, both_rows = residual && at.y;
+                auto weight = [&](int j) {
+                    if (!both_rows) return at.draw_weight(j, residual, table);
+                    const double w = fma(at.q.weight(to_f(at.y[j]), table), -at.q.iz, at.p.weight(to_f(at.x[j]), table) * at.p.iz);
+                    return w > 0 ? w : 0.0;
+                };
+                double part = 0;
+#pragma unroll 4
+                for (int j = c0 + lane; j < c1; j += 32) part += weight(j);
+                tell(warp_sum(part), 0, 0, 0);
+                // the first chunk whose running sum is above the point; with none, the last that has weight
+                const int per = (warps + 31) / 32, k0 = lane * per, k1 = k0 + 1;
+                const double t0 = k0 < warps ? told[round][k0][0] : 0.0, t1 = per > 1 && k1 < warps ? told[round][k1][0] : 0.0;
+                round ^= 1;
+                const double above = warp_scan(t0 + t1, lane), total = __shfl_sync(ALL, above, 31);
+                if (residual && !(total > RESIDUAL_MIN)) continue;
+                const double target = r * total, up = __shfl_up_sync(ALL, above, 1), before = lane ? up : 0.0;
+                unsigned cross = __ballot_sync(ALL, t0 + t1 > 0 && above > target), some = __ballot_sync(ALL, t0 + t1 > 0);
+                int owner = cross ? __ffs(cross) - 1 : 31 - __clz(some);
+                const bool second = t1 > 0 && !(t0 > 0 && before + t0 > target);
+                who = __shfl_sync(ALL, second ? k1 : k0, owner);
+                double below = __shfl_sync(ALL, second ? before + t0 : before, owner);
+                if (who != me) return;
+                // of the chunk a lane has consecutive places, of those 32 at a time one each
+                const int share = (c1 - c0 + 31) / 32;
+                int f = min(c1, c0 + lane * share);
+                const int g = min(c1, f + share);
+                part = 0;
+#pragma unroll 4
+                for (int j = f; j < g; ++j) part += weight(j);
+                const double sum = warp_scan(part, lane), lower = __shfl_up_sync(ALL, sum, 1);
+                cross = __ballot_sync(ALL, part > 0 && below + sum > target), some = __ballot_sync(ALL, part > 0);
+                owner = cross ? __ffs(cross) - 1 : 31 - __clz(some);
+                below += __shfl_sync(ALL, lane ? lower : 0.0, owner);
+                f = __shfl_sync(ALL, f, owner);
+                const int end = __shfl_sync(ALL, g, owner);
+                for (; f < end; f += 32) {
+                    const double w = f + lane < end ? weight(f + lane) : 0.0, run = warp_scan(w, lane);
+                    cross = __ballot_sync(ALL, w > 0 && below + run > target), some = __ballot_sync(ALL, w > 0);
+                    if (some) next = f + (cross ? __ffs(cross) - 1 : 31 - __clz(some));
+                    if (cross) break;
+                    below += __shfl_sync(ALL, run, 31);
                 }
-                const double target = r * total;
-                if (residual && !(total > RESIDUAL_MIN)) {
-                    round ^= 1;
-                    continue;
-                }
-                if (ranks > 1) mine = find(ranks, [&](int k) { return sm.told[round][k][0]; }, below, target) == rank;
-                if (!mine) break;
-                // an eighth of the share, of that an eighth, and so on
-                for (;;) {
-                    const int who = find(DENSE_WARPS, [&](int k) { return sm.level[k]; }, below, target);
-                    from = min(to, from + who * share), to = min(to, from + share);
-                    if (to - from <= 32) break;
-                    share = ((to - from + DENSE_WARPS - 1) / DENSE_WARPS + 31) & ~31;
-                    shares(from, to, share, residual);
-                }
-                if (warp == 0) {
-                    const int j = from + lane;
-                    const double w = j < to ? at.draw_weight(j, residual, table) : 0.0;
-                    const double above = warp_scan(w, lane);
-                    const unsigned cross = __ballot_sync(ALL, w > 0 && below + above > target), some = __ballot_sync(ALL, w > 0);
-                    if (lane == 0) sm.pick = from + (cross ? __ffs(cross) - 1 : some ? 31 - __clz(some) : 0);
-                }
-                __syncthreads();
-                next = sm.pick;
                 break;
             }
         }
-        if (!mine) return;
-        if (tid == 0) {
+        if (who != me) return;
+        if (lane == 0) {
             d.accepted[game] = i;
             out[i] = next;
             out_lp[i] = next >= 0 ? at.log_prob(next) : at.broken() ? __int_as_float(0x7fc00000) : 0.f;
         }
-        for (int k = i + 1 + tid; k <= d.drafts; k += DENSE_THREADS) out[k] = -1, out_lp[k] = 0.f;
+        for (int k = i + 1 + lane; k <= d.drafts; k += 32) out[k] = -1, out_lp[k] = 0.f;
         return;
     }
+}
+
+// Lets a kernel have `bytes` of an SM's shared memory on the current device.
+template <typename K>
+static cudaError_t allow_smem(K *kernel, int bytes, std::atomic<uint64_t> &raised) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (raised.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+template <typename T>
+static int logp_forward(LogpArgs &a, cudaStream_t s) {
+    if (!a.mask) {
+        CU(launch_pdl(logp_dense_kernel<T>, (unsigned)a.rows, LOGP_THREADS, 0, s, a));
+        return JQ_OK;
+    }
+    a.share = (int)Legal::bytes(a.n);
+    const size_t smem = (size_t)LOGP_WARPS * a.share;
+    static std::atomic<uint64_t> raised{0};
+    if (smem > 48 * 1024) CU(allow_smem(logp_masked_kernel<T>, 200 * 1024, raised));
+    CU(launch_pdl(logp_masked_kernel<T>, (unsigned)((a.rows + LOGP_WARPS - 1) / LOGP_WARPS), 32 * LOGP_WARPS, smem, s, a));
+    return JQ_OK;
+}
+
+template <typename T>
+static int logp_backward(const LogpArgs &a, cudaStream_t s) {
+    CU(a.bits ? launch_pdl(logp_bwd_kernel<T, true>, (unsigned)a.rows, LOGP_THREADS, 0, s, a)
+              : launch_pdl(logp_bwd_kernel<T, false>, (unsigned)a.rows, LOGP_THREADS, 0, s, a));
+    return JQ_OK;
 }
 
 template <typename T>
@@ -820,9 +931,9 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
     if (!d.mask) {
         int sms, rc = device_sms(sms);
         if (rc) return rc;
-        // enough CTAs for all SMs, several of which wait for one another's answers meanwhile, of a thousand places or more
+        // enough CTAs to fill the SMs once (4 each), of a thousand places or more: each place costs every warp an exchange
         int ctas = 1;
-        while (ctas < DENSE_CTAS && (int64_t)d.games * ctas < 6 * (int64_t)sms && d.actions > 1024 * ctas) ctas *= 2;
+        while (ctas < DENSE_CTAS && (int64_t)d.games * ctas < 4 * (int64_t)sms && d.actions > 1024 * ctas) ctas *= 2;
         if ((int64_t)d.games * ctas > INT32_MAX) return fail(JQ_ERR_CAPACITY, "drafts: too many games for one call");
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)d.games * ctas);
@@ -837,23 +948,17 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
         CU(cudaLaunchKernelEx(&cfg, verify_dense_kernel<T>, a));
         return JQ_OK;
     }
-    a.share = 4 * (3 * LIST + (d.actions + 15 + 31) / 32 + 1);
-    a.share = (a.share + 15) & ~15;
-    int warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
+    a.share = (int)(Legal::bytes(d.actions) + 4 * LIST * (d.draft_logits ? 2 : 1));
+    int sms, rc = device_sms(sms), warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
+    if (rc) return rc;
+    // as many places side by side as keep all games on the SMs at once (32 warps each), since the longest chain counts
+    while (warps > 2 && (int64_t)d.games * warps > 32 * (int64_t)sms) warps = (warps + 1) / 2;
     if (d.drafts == 0) warps = a.games_per_cta = 4;
     while (warps > 1 && (size_t)warps * a.share > 200 * 1024) --warps;
     if (d.drafts == 0) a.games_per_cta = warps;
     const size_t smem = (size_t)warps * a.share;
-    if (smem > 40 * 1024) {
-        static std::atomic<uint64_t> raised{0};
-        int dev = 0;
-        CU(cudaGetDevice(&dev));
-        const uint64_t bit = 1ull << (dev & 63);
-        if (!(raised.load(std::memory_order_relaxed) & bit)) {
-            CU(cudaFuncSetAttribute(verify_masked_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 210 * 1024));
-            raised.fetch_or(bit, std::memory_order_relaxed);
-        }
-    }
+    static std::atomic<uint64_t> raised{0};
+    if (smem > 40 * 1024) CU(allow_smem(verify_masked_kernel<T>, 210 * 1024, raised));
     const unsigned g = (unsigned)((d.games + a.games_per_cta - 1) / a.games_per_cta);
     CU(launch_pdl(verify_masked_kernel<T>, g, 32 * warps, smem, s, a));
     return JQ_OK;
@@ -875,21 +980,6 @@ static int logp_check(const void *x, int64_t stride, int32_t dtype, int64_t rows
     return JQ_OK;
 }
 
-#define LOGP_LAUNCH(KERNEL, MASKED)                                                                             \
-    do {                                                                                                        \
-        cudaStream_t s = (cudaStream_t)stream;                                                                  \
-        const unsigned g = (unsigned)rows;                                                                      \
-        if (dtype == JQ_F32)                                                                                    \
-            CU((MASKED) ? launch_pdl(KERNEL<float, true>, g, LOGP_THREADS, 0, s, a)                             \
-                        : launch_pdl(KERNEL<float, false>, g, LOGP_THREADS, 0, s, a));                          \
-        else if (dtype == JQ_F16)                                                                               \
-            CU((MASKED) ? launch_pdl(KERNEL<__half, true>, g, LOGP_THREADS, 0, s, a)                            \
-                        : launch_pdl(KERNEL<__half, false>, g, LOGP_THREADS, 0, s, a));                         \
-        else                                                                                                    \
-            CU((MASKED) ? launch_pdl(KERNEL<__nv_bfloat16, true>, g, LOGP_THREADS, 0, s, a)                     \
-                        : launch_pdl(KERNEL<__nv_bfloat16, false>, g, LOGP_THREADS, 0, s, a));                  \
-    } while (0)
-
 int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, const uint8_t *d_mask,
                        int64_t mask_stride, const int32_t *d_actions, int64_t rows, int32_t actions,
                        float *d_log_prob, float *d_entropy, float *d_stats, uint32_t *d_bits, void *stream) {
@@ -904,8 +994,11 @@ int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, 
     a.x = d_logits, a.mask = d_mask, a.bits = d_mask ? d_bits : nullptr, a.act = d_actions;
     a.lp = d_log_prob, a.ent = d_entropy, a.stats = (float4 *)d_stats;
     a.x_stride = row_stride, a.mask_stride = mask_stride, a.n = actions, a.words = (actions + 31) / 32;
-    LOGP_LAUNCH(logp_fwd_kernel, d_mask);
-    return JQ_OK;
+    a.rows = rows;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == JQ_F32) return logp_forward<float>(a, s);
+    if (dtype == JQ_F16) return logp_forward<__half>(a, s);
+    return logp_forward<__nv_bfloat16>(a, s);
 }
 
 int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_t dtype, const uint32_t *d_bits,
@@ -925,8 +1018,11 @@ int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_
     a.stats = (float4 *)const_cast<float *>(d_stats), a.glp = d_grad_log_prob, a.gent = d_grad_entropy;
     a.glp_stride = grad_log_prob_stride, a.gent_stride = grad_entropy_stride, a.dx = d_dlogits;
     a.x_stride = row_stride, a.n = actions, a.words = (actions + 31) / 32;
-    LOGP_LAUNCH(logp_bwd_kernel, d_bits);
-    return JQ_OK;
+    a.rows = rows;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == JQ_F32) return logp_backward<float>(a, s);
+    if (dtype == JQ_F16) return logp_backward<__half>(a, s);
+    return logp_backward<__nv_bfloat16>(a, s);
 }
 
 int jq_verify_drafts(const jq_drafts *d, void *stream) {
