@@ -96,19 +96,19 @@ __device__ __forceinline__ int pack_mask(uint16_t *bits, uint32_t *found, int mo
 }
 
 // A row's legal places, by a warp in its shared memory: the packed mask, and
-// the blocks of 16 that have some, as block << 16 | bits.  With more than LIST
-// blocks (or, for `list`, places) only the packed mask counts.  LIST is what
-// leaves room for 32 warps of verify_masked_kernel on an SM.
-constexpr int LIST = 320;
+// the blocks of 16 that have some, as block << 16 | bits, as long as there are
+// at most `most` (with more, only the packed mask counts).
+constexpr int BLOCKS = 512;  // of the log-probability: 36 warps on an SM
+constexpr int LIST = 320;    // of the verification, and the places of its list: 24 warps, as by registers
 struct Legal {
     uint32_t *found, *bits;
-    int blocks, skip, words;
-    __device__ __forceinline__ Legal(char *at) : found((uint32_t *)at), bits((uint32_t *)at + LIST) {}
-    static size_t bytes(int places) { return (4 * (LIST + (places + 15 + 31) / 32 + 1) + 15) & ~(size_t)15; }
+    int most, blocks, skip, words;
+    __device__ __forceinline__ Legal(char *bits, void *found, int most) : found((uint32_t *)found), bits((uint32_t *)bits), most(most) {}
+    static size_t bytes(int places) { return (4 * ((places + 15 + 31) / 32 + 1) + 15) & ~(size_t)15; }  // of `bits`
     __device__ __forceinline__ void read(const uint8_t *mask, int places, int lane) {
         skip = (int)((uintptr_t)mask & 15), words = (skip + places + 31) >> 5;
         __syncwarp();  // the last row's has been read
-        blocks = pack_mask((uint16_t *)bits, found, LIST, mask, places, lane);
+        blocks = pack_mask((uint16_t *)bits, found, most, mask, places, lane);
         __syncwarp();
     }
     // The places in order, as far as there are at most LIST, and their number; [w0, w1): this lane's share of the words.
@@ -116,7 +116,7 @@ struct Legal {
         const int share = (words + 31) >> 5;
         w0 = min(words, lane * share), w1 = min(words, w0 + share);
         // this lane's: of its share of the blocks that have some, or of the words
-        const bool few = blocks <= LIST;
+        const bool few = blocks <= most;
         const int per = (blocks + 31) >> 5, e0 = min(blocks, lane * per), e1 = min(blocks, e0 + per);
         int before = 0;
         if (few)
@@ -129,7 +129,7 @@ struct Legal {
             const int u = __shfl_up_sync(ALL, before, o);
             if (lane >= o) before += u;
         }
-        const int count = __shfl_sync(ALL, before, 31);  // (more than LIST blocks have more than LIST places)
+        const int count = __shfl_sync(ALL, before, 31);  // (`most` is LIST: more blocks than that have more places, too)
         before -= own;
         if (count <= LIST)
             for (int e = e0; e < e1; ++e) {
@@ -262,10 +262,10 @@ __global__ void __launch_bounds__(32 * LOGP_WARPS, 9) logp_masked_kernel(const L
     if (row >= a.rows) return;
     const T *x = (const T *)a.x + row * a.x_stride;
     const int act = a.act[row];
-    Legal legal(logp_smem + warp * a.share);
+    Legal legal(logp_smem + warp * a.share, logp_smem + (warp + 1) * a.share - 4 * BLOCKS, BLOCKS);
     legal.read(a.mask + row * a.mask_stride, a.n, lane);
     Soft acc{LOWEST, 0.f, 0.f};
-    if (legal.blocks <= LIST) {
+    if (legal.blocks <= BLOCKS) {
         // a lane's blocks, four scattered logits in flight
         uint32_t block = 0;
         for (int e = lane; e < legal.blocks || (block & 0xffff);) {
@@ -480,7 +480,7 @@ constexpr int PLACES = 8;      // of a game at the same time
 struct VerifyArgs {
     jq_drafts d;
     int32_t games_per_cta;  // masked: a game per warp, with no drafts; else 1
-    int32_t share;          // masked: bytes of shared memory of a warp
+    int32_t share, own;     // masked: bytes of shared memory of a warp, and those of them before the list
 };
 
 // e^d for d <= 0 in 64 bits: d = k ln 2 / 16 + r, e^d = 2^(k / 16) e^r, from a
@@ -507,16 +507,16 @@ __device__ __forceinline__ double exp_near(double d, const double *table) {  // 
 
 // One row of logits and what its probabilities need.
 struct Dist {
-    double m, z, iz; // the largest logit, Z and its reciprocal
-    float low;       // logits below it have exp(x - m) = 0
-    bool any;        // a legal place above -inf
-    bool broken;     // NaN or +inf at a legal place: no distribution
+    double m, z;  // the largest logit, and Z
+    float low;    // logits below it have exp(x - m) = 0
+    bool any;     // a legal place above -inf
+    bool broken;  // NaN or +inf at a legal place: no distribution
     __device__ __forceinline__ void start(float top, bool there) {
         broken = there && !(top < INFINITY);
         any = there && !broken && top > -INFINITY;
         m = any ? top : 0.f;
         low = any ? (float)(m - 700.0) : INFINITY;  // (rounded to m itself where m is beyond 2^33: the next logit is far)
-        z = iz = 0;
+        z = 0;
     }
     __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)
         const double e = exp_near((double)x - m, table);
@@ -550,22 +550,24 @@ struct Place {
         }
     }
     __device__ __forceinline__ bool broken() const { return p.broken || q.broken; }
+    // probabilities are e / Z: compared and subtracted over the common denominator, without a division
     __device__ __forceinline__ bool kept(bool legal, const double *table) const {
         if (act < 0 || !legal || broken() || !p.any) return false;
-        const double pa = p.weight(xa, table) * p.iz;
-        const double qa = !y ? 1.0 : q.any ? q.weight(ya, table) * q.iz : 0.0;
-        return (double)u * qa < pa;
+        const double ep = p.weight(xa, table);
+        if (!y) return (double)u * p.z < ep;
+        return !q.any ? 0.0 < ep : __dmul_rn((double)u * q.weight(ya, table), p.z) < __dmul_rn(ep, q.z);
     }
-    // the distribution that is drawn from: max(p - q, 0) while `residual`, else p
+    // what is drawn from, times `scale`: max(p - q, 0) while `residual`, else p; ep, eq are exp(x - m) at j
     __device__ __forceinline__ bool has_residual() const { return drafted && (y ? q.any : act >= 0); }
-    __device__ __forceinline__ double draw_weight(int j, float xj, float yj, bool residual, const double *table) const {
-        const double pj = p.weight(xj, table) * p.iz;
-        if (!residual) return pj;
-        const double qj = y ? q.weight(yj, table) * q.iz : j == act ? 1.0 : 0.0;
-        return pj > qj ? pj - qj : 0.0;
+    __device__ __forceinline__ double scale(bool residual) const { return residual && y ? p.z * q.z : p.z; }
+    __device__ __forceinline__ double draw(int j, double ep, double eq, bool residual) const {
+        if (!residual) return ep;
+        if (!y) return j == act ? 0.0 : ep;  // q is one-hot there
+        const double w = __dmul_rn(ep, q.z) - __dmul_rn(eq, p.z);
+        return w > 0 ? w : 0.0;
     }
-    __device__ __forceinline__ double draw_weight(int j, bool residual, const double *table) const {
-        return draw_weight(j, to_f(x[j]), y && residual ? to_f(y[j]) : 0.f, residual, table);
+    __device__ __forceinline__ double draw(int j, bool residual, const double *table) const {
+        return draw(j, p.weight(to_f(x[j]), table), residual && y ? q.weight(to_f(y[j]), table) : 0.0, residual);
     }
     __device__ __forceinline__ float log_prob(int j) const {  // in 64 bits, rounded once
         return (float)(((double)to_f(x[j]) - p.m) - log(p.z));
@@ -592,7 +594,7 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const VerifyArgs a) {
     extern __shared__ __align__(16) char verify_smem[];
     __shared__ double table[EXP_STEPS];
     __shared__ int keeps[2][PLACES];
@@ -601,10 +603,11 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
     for (int i = threadIdx.x; i < EXP_STEPS; i += blockDim.x) table[i] = exp_table(i);
     pdl_enter();
     __syncthreads();
-    Legal legal(verify_smem + warp * a.share);
-    // the legal actions in order and their logits (in what was scratch); the draft's, which there is room for if there are any
-    int *list = (int *)(verify_smem + (warp + 1) * a.share) - LIST;
-    float *lx = (float *)legal.found, *ly = (float *)(list - LIST);
+    // of the legal actions in order: exp(x - m), of the target and, where there are any, of the draft (until then their
+    // logits), and the actions
+    double *ep = (double *)(verify_smem + (size_t)warp * a.share + a.own), *eq = ep + LIST;
+    int *list = (int *)(d.draft_logits ? eq + LIST : eq);
+    Legal legal(verify_smem + (size_t)warp * a.share, ep, LIST);  // (the blocks found are done with when the list stands)
     const bool alone = a.games_per_cta > 1;  // a game is this warp's, and has one place
     const int game = alone ? blockIdx.x * a.games_per_cta + warp : blockIdx.x;
     if (game >= d.games) return;             // (alone: no barrier follows)
@@ -618,15 +621,15 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
         bool kept = false;
         Place<T> at(d, game, active ? i : len, len);
         int count = 0, lo = 0, hi = 0, w0 = 0, w1 = 0;
-        // this lane's legal actions, consecutive ones, with their logits: of the list, or of the packed mask
+        // this lane's legal actions, consecutive ones, with their exp(x - m): of the list, or of the packed mask
         auto each = [&](auto &&f) {
             if (count <= LIST) {
-                for (int k = lo; k < hi; ++k) f(list[k], lx[k], at.y ? ly[k] : 0.f);
+                for (int k = lo; k < hi; ++k) f(list[k], ep[k], at.y ? eq[k] : 0.0);
             } else {
                 for (int w = w0; w < w1; ++w)
                     for (uint32_t b = legal.bits[w]; b; b &= b - 1) {
                         const int j = 32 * w + __ffs(b) - 1 - legal.skip;
-                        f(j, to_f(at.x[j]), at.y ? to_f(at.y[j]) : 0.f);
+                        f(j, at.p.weight(to_f(at.x[j]), table), at.y ? at.q.weight(to_f(at.y[j]), table) : 0.0);
                     }
             }
         };
@@ -634,39 +637,61 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
             legal.read(at.mask, n, lane);
             at.fetch();
             count = legal.list(list, lane, w0, w1);
+            float mx = -INFINITY, my = -INFINITY;
+            double zx = 0, zy = 0;
             if (count <= LIST) {
                 const int per = (count + 31) >> 5;
                 lo = min(count, lane * per), hi = min(count, lo + per);
-                for (int k0 = 0; k0 < count; k0 += 128) {  // four scattered logits of each in flight
+                for (int k0 = lane; k0 < count; k0 += 128) {  // four scattered logits of each in flight
                     float vx[4], vy[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int k = k0 + 32 * i + lane;
-                        if (k < count) {
-                            vx[i] = to_f(at.x[list[k]]);
-                            if (at.y) vy[i] = to_f(at.y[list[k]]);
+                    for (int i = 0; i < 4; ++i)
+                        if (k0 + 32 * i < count) {
+                            const int j = list[k0 + 32 * i];
+                            vx[i] = to_f(at.x[j]);
+                            if (at.y) vy[i] = to_f(at.y[j]);
                         }
-                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int k = k0 + 32 * i + lane;
-                        if (k < count) lx[k] = vx[i];
-                        if (k < count && at.y) ly[k] = vy[i];
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (k0 + 32 * i < count) {
+                            mx = max_nan(mx, vx[i]);
+                            *(float *)(ep + k0 + 32 * i) = vx[i];
+                            if (at.y) {
+                                my = max_nan(my, vy[i]);
+                                *(float *)(eq + k0 + 32 * i) = vy[i];
+                            }
+                        }
                 }
-                __syncwarp();
+            } else {
+                for (int w = 0; w < legal.words; ++w)  // many: a lane per place
+                    if ((legal.bits[w] >> lane) & 1) {
+                        mx = max_nan(mx, to_f(at.x[32 * w + lane - legal.skip]));
+                        if (at.y) my = max_nan(my, to_f(at.y[32 * w + lane - legal.skip]));
+                    }
             }
-            float mx = -INFINITY, my = -INFINITY;
-            each([&](int, float x, float y) { mx = max_nan(mx, x), my = max_nan(my, y); });
             at.p.start(warp_max(mx), true);
             at.q.start(warp_max(my), at.y != nullptr);
-            double zx = 0, zy = 0;
-            each([&](int, float x, float y) {
-                zx += at.p.weight(x, table);
-                if (at.y) zy += at.q.weight(y, table);
-            });
-            at.p.z = warp_sum(zx), at.q.z = warp_sum(zy);
-            at.p.iz = 1.0 / at.p.z, at.q.iz = 1.0 / at.q.z;
+            if (count <= LIST) {
+#pragma unroll 2
+                for (int k = lane; k < count; k += 32) {
+                    const double e = at.p.weight(*(float *)(ep + k), table);
+                    ep[k] = e, zx += e;
+                    if (at.y) {
+                        const double g = at.q.weight(*(float *)(eq + k), table);
+                        eq[k] = g, zy += g;
+                    }
+                }
+            } else {
+                for (int w = 0; w < legal.words; ++w)
+                    if ((legal.bits[w] >> lane) & 1) {
+                        zx += at.p.weight(to_f(at.x[32 * w + lane - legal.skip]), table);
+                        if (at.y) zy += at.q.weight(to_f(at.y[32 * w + lane - legal.skip]), table);
+                    }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) zx += __shfl_xor_sync(ALL, zx, o), zy += __shfl_xor_sync(ALL, zy, o);
+            at.p.z = zx, at.q.z = zy;
+            __syncwarp();  // the list's exponentials are read by other lanes
             kept = at.kept(at.act >= 0 && legal.has(at.act), table);
         }
         int first = alone ? 0 : warps;  // the first place of this round that is not kept
@@ -686,9 +711,9 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
                 const bool residual = pass == 0;
                 double part = 0;
-                each([&](int j, float x, float y) { part += at.draw_weight(j, x, y, residual, table); });
+                each([&](int j, double p, double q) { part += at.draw(j, p, q, residual); });
                 const double above = warp_scan(part, lane), total = __shfl_sync(ALL, above, 31);
-                if (residual && !(total > RESIDUAL_MIN)) continue;
+                if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
                 const double up = __shfl_up_sync(ALL, above, 1), below = lane ? up : 0.0, target = r * total;
                 // the first lane whose running sum is above the point; with none, the last that has weight
                 const unsigned cross = __ballot_sync(ALL, part > 0 && above > target), some = __ballot_sync(ALL, part > 0);
@@ -696,8 +721,8 @@ __global__ void __launch_bounds__(32 * PLACES, 4) verify_masked_kernel(const Ver
                 if (lane == who) {
                     double run = below;
                     bool crossed = false;
-                    each([&](int j, float x, float y) {
-                        const double w = at.draw_weight(j, x, y, residual, table);
+                    each([&](int j, double p, double q) {
+                        const double w = at.draw(j, p, q, residual);
                         run += w;
                         if (w > 0 && !crossed) next = j, crossed = run > target;
                     });
@@ -817,11 +842,11 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
             at.q.start(warp_max(max_nan(q0, q1)), at.y != nullptr);
             double z = lane < warps ? told[round][lane][1] * at.p.weight(m0, table) : 0.0;
             if (k1 < warps) z += told[round][k1][1] * at.p.weight(m1, table);
-            at.p.z = warp_sum(z), at.p.iz = 1.0 / at.p.z;
+            at.p.z = warp_sum(z);
             if (at.y) {
                 z = lane < warps ? told[round][lane][3] * at.q.weight(q0, table) : 0.0;
                 if (k1 < warps) z += told[round][k1][3] * at.q.weight(q1, table);
-                at.q.z = warp_sum(z), at.q.iz = 1.0 / at.q.z;
+                at.q.z = warp_sum(z);
             }
             round ^= 1;
         }
@@ -834,12 +859,8 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
-                const bool residual = pass == 0, both_rows = residual && at.y;
-                auto weight = [&](int j) {
-                    if (!both_rows) return at.draw_weight(j, residual, table);
-                    const double w = fma(at.q.weight(to_f(at.y[j]), table), -at.q.iz, at.p.weight(to_f(at.x[j]), table) * at.p.iz);
-                    return w > 0 ? w : 0.0;
-                };
+                const bool residual = pass == 0;
+                auto weight = [&](int j) { return at.draw(j, residual, table); };
                 double part = 0;
 #pragma unroll 4
                 for (int j = c0 + lane; j < c1; j += 32) part += weight(j);
@@ -849,7 +870,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
                 const double t0 = k0 < warps ? told[round][k0][0] : 0.0, t1 = per > 1 && k1 < warps ? told[round][k1][0] : 0.0;
                 round ^= 1;
                 const double above = warp_scan(t0 + t1, lane), total = __shfl_sync(ALL, above, 31);
-                if (residual && !(total > RESIDUAL_MIN)) continue;
+                if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
                 const double target = r * total, up = __shfl_up_sync(ALL, above, 1), before = lane ? up : 0.0;
                 unsigned cross = __ballot_sync(ALL, t0 + t1 > 0 && above > target), some = __ballot_sync(ALL, t0 + t1 > 0);
                 int owner = cross ? __ffs(cross) - 1 : 31 - __clz(some);
@@ -910,7 +931,7 @@ static int logp_forward(LogpArgs &a, cudaStream_t s) {
         CU(launch_pdl(logp_dense_kernel<T>, (unsigned)a.rows, LOGP_THREADS, 0, s, a));
         return JQ_OK;
     }
-    a.share = (int)Legal::bytes(a.n);
+    a.share = (int)Legal::bytes(a.n) + 4 * BLOCKS;
     const size_t smem = (size_t)LOGP_WARPS * a.share;
     static std::atomic<uint64_t> raised{0};
     if (smem > 48 * 1024) CU(allow_smem(logp_masked_kernel<T>, 200 * 1024, raised));
@@ -927,7 +948,7 @@ static int logp_backward(const LogpArgs &a, cudaStream_t s) {
 
 template <typename T>
 static int verify_launch(const jq_drafts &d, cudaStream_t s) {
-    VerifyArgs a{d, 1, 0};
+    VerifyArgs a{d, 1, 0, 0};
     if (!d.mask) {
         int sms, rc = device_sms(sms);
         if (rc) return rc;
@@ -948,11 +969,12 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
         CU(cudaLaunchKernelEx(&cfg, verify_dense_kernel<T>, a));
         return JQ_OK;
     }
-    a.share = (int)(Legal::bytes(d.actions) + 4 * LIST * (d.draft_logits ? 2 : 1));
+    a.own = (int)Legal::bytes(d.actions);
+    a.share = a.own + LIST * (d.draft_logits ? 20 : 12);
     int sms, rc = device_sms(sms), warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
     if (rc) return rc;
-    // as many places side by side as keep all games on the SMs at once (32 warps each), since the longest chain counts
-    while (warps > 2 && (int64_t)d.games * warps > 32 * (int64_t)sms) warps = (warps + 1) / 2;
+    // as many places side by side as keep all games on the SMs at once (24 warps each), since the longest chain counts
+    while (warps > 2 && (int64_t)d.games * warps > 24 * (int64_t)sms) --warps;
     if (d.drafts == 0) warps = a.games_per_cta = 4;
     while (warps > 1 && (size_t)warps * a.share > 200 * 1024) --warps;
     if (d.drafts == 0) a.games_per_cta = warps;
