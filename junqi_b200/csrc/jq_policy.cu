@@ -479,7 +479,6 @@ constexpr int PLACES = 8;      // of a game at the same time
 
 struct VerifyArgs {
     jq_drafts d;
-    int32_t games_per_cta;  // masked: a game per warp, with no drafts; else 1
     int32_t share, own;     // masked: bytes of shared memory of a warp, and those of them before the list
 };
 
@@ -507,15 +506,14 @@ __device__ __forceinline__ double exp_near(double d, const double *table) {  // 
 
 // One row of logits and what its probabilities need.
 struct Dist {
+    enum { NONE = 0, SOME = 1, BROKEN = 2 };  // no legal place above -inf; a distribution; NaN or +inf at a legal place
     double m, z;  // the largest logit, and Z
     float low;    // logits below it have exp(x - m) = 0
-    bool any;     // a legal place above -inf
-    bool broken;  // NaN or +inf at a legal place: no distribution
+    int state;
     __device__ __forceinline__ void start(float top, bool there) {
-        broken = there && !(top < INFINITY);
-        any = there && !broken && top > -INFINITY;
-        m = any ? top : 0.f;
-        low = any ? (float)(m - 700.0) : INFINITY;  // (rounded to m itself where m is beyond 2^33: the next logit is far)
+        state = !there || top == -INFINITY ? NONE : top < INFINITY ? SOME : BROKEN;
+        m = state == SOME ? top : 0.f;
+        low = state == SOME ? (float)(m - 700.0) : INFINITY;  // (rounded to m itself where m is beyond 2^33: the next logit is far)
         z = 0;
     }
     __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)
@@ -549,16 +547,16 @@ struct Place {
             if (y) ya = to_f(y[act]);
         }
     }
-    __device__ __forceinline__ bool broken() const { return p.broken || q.broken; }
+    __device__ __forceinline__ bool broken() const { return (p.state | q.state) & Dist::BROKEN; }
     // probabilities are e / Z: compared and subtracted over the common denominator, without a division
     __device__ __forceinline__ bool kept(bool legal, const double *table) const {
-        if (act < 0 || !legal || broken() || !p.any) return false;
+        if (act < 0 || !legal || broken() || p.state != Dist::SOME) return false;
         const double ep = p.weight(xa, table);
         if (!y) return (double)u * p.z < ep;
-        return !q.any ? 0.0 < ep : __dmul_rn((double)u * q.weight(ya, table), p.z) < __dmul_rn(ep, q.z);
+        return q.state != Dist::SOME ? 0.0 < ep : __dmul_rn((double)u * q.weight(ya, table), p.z) < __dmul_rn(ep, q.z);
     }
     // what is drawn from, times `scale`: max(p - q, 0) while `residual`, else p; ep, eq are exp(x - m) at j
-    __device__ __forceinline__ bool has_residual() const { return drafted && (y ? q.any : act >= 0); }
+    __device__ __forceinline__ bool has_residual() const { return drafted && (y ? q.state == Dist::SOME : act >= 0); }
     __device__ __forceinline__ double scale(bool residual) const { return residual && y ? p.z * q.z : p.z; }
     __device__ __forceinline__ double draw(int j, double ep, double eq, bool residual) const {
         if (!residual) return ep;
@@ -593,8 +591,9 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
     return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const VerifyArgs a) {
+// ALONE: no drafts, a game per warp.
+template <typename T, bool ALONE>
+__global__ void __launch_bounds__(ALONE ? 128 : 32 * PLACES, ALONE ? 8 : 3) verify_masked_kernel(const VerifyArgs a) {
     extern __shared__ __align__(16) char verify_smem[];
     __shared__ double table[EXP_STEPS];
     __shared__ int keeps[2][PLACES];
@@ -606,20 +605,23 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
     // of the legal actions in order: exp(x - m), of the target and, where there are any, of the draft (until then their
     // logits), and the actions
     double *ep = (double *)(verify_smem + (size_t)warp * a.share + a.own), *eq = ep + LIST;
-    int *list = (int *)(d.draft_logits ? eq + LIST : eq);
+    int *list = (int *)(!ALONE && d.draft_logits ? eq + LIST : eq);
     Legal legal(verify_smem + (size_t)warp * a.share, ep, LIST);  // (the blocks found are done with when the list stands)
-    const bool alone = a.games_per_cta > 1;  // a game is this warp's, and has one place
-    const int game = alone ? blockIdx.x * a.games_per_cta + warp : blockIdx.x;
-    if (game >= d.games) return;             // (alone: no barrier follows)
-    int len = d.lengths ? d.lengths[game] : d.drafts;
-    len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
+    const int game = ALONE ? blockIdx.x * warps + warp : blockIdx.x;
+    if (game >= d.games) return;  // (ALONE: no barrier follows)
+    int len = 0;
+    if (!ALONE) {
+        len = d.lengths ? d.lengths[game] : d.drafts;
+        len = len < 0 ? 0 : len > d.drafts ? d.drafts : len;
+    }
     int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
     float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
     for (int base = 0, round = 0;; base += warps, round ^= 1) {
-        const int i = alone ? 0 : base + warp;
+        const int i = ALONE ? 0 : base + warp;
         const bool active = i <= len;
         bool kept = false;
         Place<T> at(d, game, active ? i : len, len);
+        if (ALONE) at.y = nullptr, at.act = -1, at.drafted = false;
         int count = 0, lo = 0, hi = 0, w0 = 0, w1 = 0;
         // this lane's legal actions, consecutive ones, with their exp(x - m): of the list, or of the packed mask
         auto each = [&](auto &&f) {
@@ -655,10 +657,10 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
                     for (int i = 0; i < 4; ++i)
                         if (k0 + 32 * i < count) {
                             mx = max_nan(mx, vx[i]);
-                            *(float *)(ep + k0 + 32 * i) = vx[i];
+                            ep[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vx[i]));
                             if (at.y) {
                                 my = max_nan(my, vy[i]);
-                                *(float *)(eq + k0 + 32 * i) = vy[i];
+                                eq[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vy[i]));
                             }
                         }
                 }
@@ -674,10 +676,10 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
             if (count <= LIST) {
 #pragma unroll 2
                 for (int k = lane; k < count; k += 32) {
-                    const double e = at.p.weight(*(float *)(ep + k), table);
+                    const double e = at.p.weight(__int_as_float(__double2loint(ep[k])), table);
                     ep[k] = e, zx += e;
                     if (at.y) {
-                        const double g = at.q.weight(*(float *)(eq + k), table);
+                        const double g = at.q.weight(__int_as_float(__double2loint(eq[k])), table);
                         eq[k] = g, zy += g;
                     }
                 }
@@ -694,8 +696,8 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
             __syncwarp();  // the list's exponentials are read by other lanes
             kept = at.kept(at.act >= 0 && legal.has(at.act), table);
         }
-        int first = alone ? 0 : warps;  // the first place of this round that is not kept
-        if (!alone) {
+        int first = ALONE ? 0 : warps;  // the first place of this round that is not kept
+        if (!ALONE) {
             if (lane == 0) keeps[round][warp] = kept;
             __syncthreads();
             for (int k = warps - 1; k >= 0; --k)
@@ -705,15 +707,14 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
             if (warp != first) return;
         }
         int next = -1;
-        if (at.p.any && !at.broken()) {
+        if (at.p.state == Dist::SOME && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
-            for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
-                const bool residual = pass == 0;
+            auto draw = [&](bool residual) {  // false: nothing left to draw from
                 double part = 0;
                 each([&](int j, double p, double q) { part += at.draw(j, p, q, residual); });
                 const double above = warp_scan(part, lane), total = __shfl_sync(ALL, above, 31);
-                if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
+                if (residual && !(total > RESIDUAL_MIN * at.scale(true))) return false;
                 const double up = __shfl_up_sync(ALL, above, 1), below = lane ? up : 0.0, target = r * total;
                 // the first lane whose running sum is above the point; with none, the last that has weight
                 const unsigned cross = __ballot_sync(ALL, part > 0 && above > target), some = __ballot_sync(ALL, part > 0);
@@ -728,8 +729,9 @@ __global__ void __launch_bounds__(32 * PLACES, 3) verify_masked_kernel(const Ver
                     });
                 }
                 next = __shfl_sync(ALL, next, who);
-                break;
-            }
+                return true;
+            };
+            if (ALONE || !at.has_residual() || !draw(true)) draw(false);
         }
         if (lane == 0) {
             d.accepted[game] = i;
@@ -784,7 +786,7 @@ __device__ __forceinline__ float dense_top(const T *x, int n, int lane) {
 template <typename T>
 __device__ __forceinline__ double dense_sum(const T *x, int n, int lane, const Dist &d, const double *table) {
     double z = 0;
-    if (d.any) dense_each(x, n, lane, [&](float v) { z += d.weight(v, table); });
+    if (d.state == Dist::SOME) dense_each(x, n, lane, [&](float v) { z += d.weight(v, table); });
     return z;
 }
 
@@ -855,7 +857,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
             continue;
         }
         int next = -1, who = 0;  // who: the warp whose chunk has the point
-        if (at.p.any && !at.broken()) {
+        if (at.p.state == Dist::SOME && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
@@ -948,7 +950,7 @@ static int logp_backward(const LogpArgs &a, cudaStream_t s) {
 
 template <typename T>
 static int verify_launch(const jq_drafts &d, cudaStream_t s) {
-    VerifyArgs a{d, 1, 0, 0};
+    VerifyArgs a{d, 0, 0};
     if (!d.mask) {
         int sms, rc = device_sms(sms);
         if (rc) return rc;
@@ -970,19 +972,22 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
         return JQ_OK;
     }
     a.own = (int)Legal::bytes(d.actions);
-    a.share = a.own + LIST * (d.draft_logits ? 20 : 12);
+    a.share = a.own + LIST * (d.draft_logits && d.drafts ? 20 : 12);
+    static std::atomic<uint64_t> raised[2];
+    if (d.drafts == 0) {
+        int warps = 4;
+        while (warps > 1 && warps * a.share > 200 * 1024) --warps;
+        if (warps * a.share > 40 * 1024) CU(allow_smem(verify_masked_kernel<T, true>, 210 * 1024, raised[1]));
+        CU(launch_pdl(verify_masked_kernel<T, true>, (unsigned)((d.games + warps - 1) / warps), 32 * warps, warps * a.share, s, a));
+        return JQ_OK;
+    }
     int sms, rc = device_sms(sms), warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
     if (rc) return rc;
     // as many places side by side as keep all games on the SMs at once (24 warps each), since the longest chain counts
     while (warps > 2 && (int64_t)d.games * warps > 24 * (int64_t)sms) --warps;
-    if (d.drafts == 0) warps = a.games_per_cta = 4;
-    while (warps > 1 && (size_t)warps * a.share > 200 * 1024) --warps;
-    if (d.drafts == 0) a.games_per_cta = warps;
-    const size_t smem = (size_t)warps * a.share;
-    static std::atomic<uint64_t> raised{0};
-    if (smem > 40 * 1024) CU(allow_smem(verify_masked_kernel<T>, 210 * 1024, raised));
-    const unsigned g = (unsigned)((d.games + a.games_per_cta - 1) / a.games_per_cta);
-    CU(launch_pdl(verify_masked_kernel<T>, g, 32 * warps, smem, s, a));
+    while (warps > 1 && warps * a.share > 200 * 1024) --warps;
+    if (warps * a.share > 40 * 1024) CU(allow_smem(verify_masked_kernel<T, false>, 210 * 1024, raised[0]));
+    CU(launch_pdl(verify_masked_kernel<T, false>, (unsigned)d.games, 32 * warps, warps * a.share, s, a));
     return JQ_OK;
 }
 
