@@ -7,11 +7,13 @@ status, a ``RuntimeError`` carrying ``jq_last_error()`` is raised.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import subprocess
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libjq.so"
+POLICY_PATH = _PKG / "_policy.so"  # the policy operators' torch binding (csrc/jq_torch.cpp)
 TRACE_LIB_PATH = _PKG / "libjq_trace.so"  # the same library with kernel timestamps (make -C csrc trace)
 CSRC = _PKG / "csrc"
 
@@ -119,12 +121,15 @@ SIGNATURES = {
 
 
 def build(force: bool = False, trace: bool = False) -> Path:
-    """Compile libjq.so (or, with ``trace``, libjq_trace.so) for sm_100a with
-    nvcc (csrc/Makefile)."""
+    """Compile libjq.so and _policy.so (or, with ``trace``, libjq_trace.so) for
+    sm_100a with nvcc and the host compiler (csrc/Makefile)."""
     path = TRACE_LIB_PATH if trace else LIB_PATH
-    srcs = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + \
-        [_PKG.parent / "include" / "jq.h"]
-    stale = not path.exists() or any(p.stat().st_mtime > path.stat().st_mtime for p in srcs)
+    header = _PKG.parent / "include" / "jq.h"
+    need = {path: list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [header]}
+    if not trace:
+        need[POLICY_PATH] = list(CSRC.glob("*.cpp")) + [header]
+    stale = any(not out.exists() or any(p.stat().st_mtime > out.stat().st_mtime for p in srcs)
+                for out, srcs in need.items())
     if force or stale:
         subprocess.run(["make", "-s", "-C", str(CSRC)] + (["trace"] if trace else []), check=True)
     return path
@@ -156,6 +161,26 @@ def lib():
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_policy = None
+
+
+def policy():
+    """Load _policy.so (raising if it is absent), bound to the loaded library's entry points."""
+    global _policy
+    if _policy is None:
+        if not POLICY_PATH.exists():
+            raise RuntimeError(f"{POLICY_PATH.name} not built at {POLICY_PATH}; run junqi_b200._native.build()")
+        L = lib()
+        spec = importlib.util.spec_from_file_location("junqi_b200._policy", POLICY_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in (
+            "jq_last_error", "jq_layer_norm", "jq_layer_norm_scratch_floats", "jq_layer_norm_backward",
+            "jq_action_log_prob", "jq_action_log_prob_backward", "jq_verify_drafts")})
+        _policy = mod
+    return _policy
 
 
 def check(status: int, what: str) -> None:

@@ -383,6 +383,48 @@ def test_action_log_prob_actions_without_a_value():
     assert not d1.any()
 
 
+@pytest.mark.parametrize("kind", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_whole_numbers_of_any_type_and_none_wraps(kind):
+    """2^32 + 5 is not action 5, and -2^40 not action 0, in any argument of 64 bits."""
+    x = torch.randn(4, 2, 90, generator=gen(1), device="cuda")
+    a = torch.tensor([5, 0, 89, 7], device="cuda")
+    want = P.action_log_prob(x[:, 0], None, a)[0]
+    assert torch.equal(P.action_log_prob(x[:, 0], None, a.to(kind))[0], want)
+    if kind == torch.int64:
+        far = torch.tensor([2 ** 32 + 5, -2 ** 40, 89, 2 ** 40 + 7], device="cuda")
+        lp, _ = P.action_log_prob(x[:, 0], None, far)
+        assert lp[[0, 1, 3]].tolist() == [0, 0, 0] and lp[2] == want[2]
+        v = P.verify_drafts(x, far[:, None], torch.zeros(4, 1, device="cuda"), torch.zeros(4, device="cuda"),
+                            lengths=torch.tensor([2 ** 32, 2 ** 32 + 1, -2 ** 33, 1], device="cuda"))
+        assert v.accepted.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("op", ["norm", "logp"])
+def test_second_derivatives_are_refused(op):
+    x = torch.randn(3, 20, generator=gen(1), device="cuda", requires_grad=True)
+    if op == "norm":
+        y = P.layer_norm(x).square().sum()
+    else:
+        y = P.action_log_prob(x, None, torch.zeros(3, dtype=torch.int32, device="cuda"))[0].square().sum()
+    (g,) = torch.autograd.grad(y, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_results_do_not_need_gradients_where_nothing_asks_for_them():
+    x = torch.randn(3, 20, device="cuda", requires_grad=True)
+    a = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        assert not P.layer_norm(x).requires_grad and not P.action_log_prob(x, None, a)[0].requires_grad
+    assert not P.layer_norm(x.detach()).requires_grad
+    s, lp = P.sample_actions(x, None, torch.rand(3, device="cuda"))
+    assert not lp.requires_grad
+    w = torch.ones(20, device="cuda", requires_grad=True)
+    y = P.layer_norm(x.detach(), w)
+    (gw,) = torch.autograd.grad(y.sum(), w)
+    assert gw.shape == (20,)
+
+
 def test_action_log_prob_one_gradient_only_and_broadcast_gradients():
     x = torch.randn(2, 5, 90, generator=gen(8), device="cuda", requires_grad=True)
     m = torch.rand(90, generator=gen(9), device="cuda") < 0.5

@@ -95,11 +95,6 @@ def test_sample_actions_refuses(args, text):
         P.sample_actions(*args)
 
 
-def test_whole_numbers_beyond_32_bits_do_not_wrap():
-    a = torch.tensor([2 ** 32 + 5, -2 ** 40, 3, -1])
-    assert P._int32("a", a, (4,), -1, 10).tolist() == [10, -1, 3, -1]
-
-
 def _status(name, *args):
     return getattr(N.lib(), name)(*args), N.lib().jq_last_error().decode()
 
