@@ -394,9 +394,11 @@ int jq_layer_norm_backward(const void *d_x, int64_t x_stride, const void *d_weig
  * not looked at.  An action outside [0, actions) is "no action": 0.  One
  * that is not legal, or whose logit is -inf: -inf.  A row without a legal
  * place above -inf has entropy 0.  NaN or +inf at a legal place: NaN.
- * For the backward pass: d_stats (rows x 4 floats, 16-byte aligned) and, with
- * a mask, d_bits (rows x ceil(actions / 32) words), the mask in bits; both
- * NULL when there will be none. */
+ * For the backward pass: d_stats (rows x 4 floats, 16-byte aligned; the action
+ * among them) and, with a mask, d_bits (rows x ceil(actions / 32) words), the
+ * mask in bits: it reads neither d_mask nor d_actions again, which may be
+ * buffers of the environment or the collector.  Both NULL when there will be
+ * none. */
 int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, const uint8_t *d_mask,
                        int64_t mask_stride, const int32_t *d_actions, int64_t rows, int32_t actions,
                        float *d_log_prob, float *d_entropy, float *d_stats, uint32_t *d_bits, void *stream);
@@ -406,10 +408,9 @@ int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, 
  * NULL: 0).  d_bits NULL: there was no mask.  A log-probability that does not
  * depend on the logits (no action, or -inf) has no gradient. */
 int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_t dtype, const uint32_t *d_bits,
-                                const int32_t *d_actions, const float *d_stats, const float *d_grad_log_prob,
-                                int64_t grad_log_prob_stride, const float *d_grad_entropy,
-                                int64_t grad_entropy_stride, int64_t rows, int32_t actions, void *d_dlogits,
-                                void *stream);
+                                const float *d_stats, const float *d_grad_log_prob, int64_t grad_log_prob_stride,
+                                const float *d_grad_entropy, int64_t grad_entropy_stride, int64_t rows,
+                                int32_t actions, void *d_dlogits, void *stream);
 
 /* Verification of drafted actions against a target policy, from given random
  * numbers in [0, 1).  Per game, with p_i the target's probabilities at place

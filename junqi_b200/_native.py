@@ -113,8 +113,8 @@ SIGNATURES = {
     "jq_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp,
                                               _vp, _vp]),
     "jq_action_log_prob": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),
-    "jq_action_log_prob_backward": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i32,
-                                                   _vp, _vp]),
+    "jq_action_log_prob_backward": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i32, _vp,
+                                                   _vp]),
     "jq_verify_drafts": (ctypes.c_int, [ctypes.POINTER(JqDrafts), _vp]),
     "jq_trace_read": (ctypes.c_int, [_i32, _vp, _i32]),
 }

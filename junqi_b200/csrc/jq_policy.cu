@@ -220,7 +220,7 @@ struct LogpArgs {
     uint32_t *bits;        // (rows, words): the packed mask; written by the forward pass (may be NULL there)
     const int32_t *act;
     float *lp, *ent;       // forward outputs
-    float4 *stats;         // (rows): m, 1 / Z, log Z, H
+    float4 *stats;         // (rows): m, 1 / Z, H - log Z, and the action's bits
     const float *glp, *gent;
     void *dx;
     int64_t rows, x_stride, mask_stride, glp_stride, gent_stride;
@@ -241,7 +241,7 @@ __device__ __forceinline__ void logp_finish(const LogpArgs &a, int64_t row, cons
     }
     a.lp[row] = lp;
     a.ent[row] = h;
-    if (a.stats) a.stats[row] = make_float4(acc.m, inv, logz, h);
+    if (a.stats) a.stats[row] = make_float4(acc.m, inv, h - logz, __int_as_float(act));
 }
 
 __device__ __forceinline__ void warp_join(Soft &acc) {
@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
     const int tid = threadIdx.x, lane = tid & 31;
     const uint32_t *bits = MASK ? a.bits + row * a.words : nullptr;
     uint32_t mine = MASK && tid < a.words ? bits[tid] : 0, more = MASK && tid + LOGP_THREADS < a.words ? bits[tid + LOGP_THREADS] : 0;
-    const float4 st = a.stats[row];  // m, 1 / Z, log Z, H
-    const int act = a.act[row];
+    const float4 st = a.stats[row];  // m, 1 / Z, H - log Z, the action
+    const int act = __float_as_int(st.w);
     const bool inside = act >= 0 && act < a.n;
     const bool legal = inside && (!MASK || ((bits[act >> 5] >> (act & 31)) & 1));
     const float xa = inside ? to_f(x[act]) : 0.f;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
         if (tid < rest) dx[tid < head ? tid : tid + packs * VEC] = zero.v[0];
         // the action's gradient: none without an action, or with one whose log-probability is -inf
         if (!legal || xa == -INFINITY) u = 0.f;
-        k0 = -(u + v * (st.w - st.z)) * st.y;
+        k0 = -(u + v * st.z) * st.y;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
         }
     } else {
         if (!legal || xa == -INFINITY) u = 0.f;
-        k0 = -(u + v * (st.w - st.z)) * st.y;
+        k0 = -(u + v * st.z) * st.y;
         const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;  // x's packs start where dx's do
         const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
         const f2 nm = both(-st.x), l = both(LOG2E), f0 = both(k0), f1 = both(k1);
@@ -1029,23 +1029,21 @@ int jq_action_log_prob(const void *d_logits, int64_t row_stride, int32_t dtype, 
 }
 
 int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_t dtype, const uint32_t *d_bits,
-                                const int32_t *d_actions, const float *d_stats, const float *d_grad_log_prob,
-                                int64_t grad_log_prob_stride, const float *d_grad_entropy,
-                                int64_t grad_entropy_stride, int64_t rows, int32_t actions, void *d_dlogits,
-                                void *stream) {
+                                const float *d_stats, const float *d_grad_log_prob, int64_t grad_log_prob_stride,
+                                const float *d_grad_entropy, int64_t grad_entropy_stride, int64_t rows,
+                                int32_t actions, void *d_dlogits, void *stream) {
     int rc = logp_check(d_logits, row_stride, dtype, rows, actions);
     if (rc) return rc;
-    if (!d_actions || !d_stats || !d_dlogits) return fail(JQ_ERR_ARG, "action scores: actions, statistics or output missing");
+    if (!d_stats || !d_dlogits) return fail(JQ_ERR_ARG, "action scores: statistics or output missing");
     if (grad_log_prob_stride < 0 || grad_entropy_stride < 0) return fail(JQ_ERR_ARG, "action scores: negative stride");
-    if (((uintptr_t)d_actions | (uintptr_t)d_bits | (uintptr_t)d_grad_log_prob | (uintptr_t)d_grad_entropy) & 3 ||
-        (uintptr_t)d_stats & 15 || (uintptr_t)d_dlogits & (elem_size(dtype) - 1))
+    if (((uintptr_t)d_bits | (uintptr_t)d_grad_log_prob | (uintptr_t)d_grad_entropy) & 3 || (uintptr_t)d_stats & 15 ||
+        (uintptr_t)d_dlogits & (elem_size(dtype) - 1))
         return fail(JQ_ERR_ARG, "action scores: an array is not aligned to its elements");
     LogpArgs a{};
-    a.x = d_logits, a.bits = const_cast<uint32_t *>(d_bits), a.act = d_actions;
+    a.x = d_logits, a.bits = const_cast<uint32_t *>(d_bits);
     a.stats = (float4 *)const_cast<float *>(d_stats), a.glp = d_grad_log_prob, a.gent = d_grad_entropy;
     a.glp_stride = grad_log_prob_stride, a.gent_stride = grad_entropy_stride, a.dx = d_dlogits;
-    a.x_stride = row_stride, a.n = actions, a.words = (actions + 31) / 32;
-    a.rows = rows;
+    a.rows = rows, a.x_stride = row_stride, a.n = actions, a.words = (actions + 31) / 32;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == JQ_F32) return logp_backward<float>(a, s);
     if (dtype == JQ_F16) return logp_backward<__half>(a, s);

@@ -87,7 +87,8 @@ Tensor rows_of(const Tensor &t) { return last(t.dim() == 2 ? t : t.reshape({-1, 
 
 // `t` as contiguous int32 of `shape`; 64-bit values are cut to [lo, hi] first, so that none wraps.
 Tensor ints(const char *what, const Tensor &t, at::IntArrayRef shape, int64_t lo, int64_t hi) {
-    REQUIRE(at::isIntegralType(t.scalar_type(), false), what, " must be whole numbers, got ", t.scalar_type());
+    const auto k = t.scalar_type();
+    REQUIRE(k == at::kInt || k == at::kLong || k == at::kShort || k == at::kChar || k == at::kByte, what, " must be whole numbers, got ", t.scalar_type());
     REQUIRE(t.sizes() == shape, what, " must be ", shape_of(shape), ", got ", shape_of(t.sizes()));
     if (t.scalar_type() == at::kInt) return t.contiguous();
     return (t.scalar_type() == at::kLong ? t.clamp(lo, hi) : t).to(at::kInt).contiguous();
@@ -233,14 +234,14 @@ struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
         const int64_t rows = x2.size(0), n = x2.size(1);
         const Tensor stats = at::empty({rows, 4}, logits.options().dtype(at::kFloat));
         const Tensor bits = mask ? at::empty({rows, (n + 31) / 32}, logits.options().dtype(at::kInt)) : Tensor();
-        ctx->save_for_backward({x2, act, stats, bits});
+        ctx->save_for_backward({x2, stats, bits});
         ctx->set_materialize_grads(false);
         auto [lp, ent] = logp_forward(logits, x2, m2, act, stats, bits);
         return {lp, ent};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x2 = saved[0], &act = saved[1], &stats = saved[2], &bits = saved[3];
+        const Tensor &x2 = saved[0], &stats = saved[1], &bits = saved[2];
         const Tensor &some = grads[0].defined() ? grads[0] : grads[1];
         if (!some.defined()) return {Tensor(), Tensor(), Tensor()};
         Tensor dx;
@@ -252,7 +253,7 @@ struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
             if (x2.size(0) > 0) {
                 On on(x2);
                 const Tensor u = grads[0].defined() ? grads[0].reshape({-1}) : Tensor(), v = grads[1].defined() ? grads[1].reshape({-1}) : Tensor();
-                check(api.log_prob_backward(ptr(x2), x2.stride(0), dtype_of("logits", x2), ptr<uint32_t>(bits), ptr<int32_t>(act),
+                check(api.log_prob_backward(ptr(x2), x2.stride(0), dtype_of("logits", x2), ptr<uint32_t>(bits),
                                             ptr<float>(stats), ptr<float>(u), u.defined() ? u.stride(0) : 0, ptr<float>(v),
                                             v.defined() ? v.stride(0) : 0, x2.size(0), (int32_t)x2.size(1), ptr(dx), on.stream),
                       "jq_action_log_prob_backward");

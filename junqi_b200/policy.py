@@ -14,9 +14,10 @@ these are the hand-written CUDA operators in between (``jq_layer_norm``,
   is a policy for :class:`junqi_b200.collector.RolloutCollector`.
 
 Logits and features are float32, float16 or bfloat16; masks are the
-environment's own (uint8 or bool, nonzero: legal), or None.  A mask is read
-during the call: the environment's and the history's masks are buffers that
-their next call overwrites, so the backward pass keeps its own copy, in bits.
+environment's own (uint8 or bool, nonzero: legal), or None.  Masks and actions
+are read during the call: those of the environment, the history and the
+collector are buffers that their next call overwrites, so the backward pass
+keeps its own copy, the mask's in bits.
 Everything runs on the current stream of the tensors' device, synchronises
 nothing, and may be captured into a CUDA graph.  A backward pass that is
 captured needs leaves that no earlier eager graph still refers to: release

@@ -477,14 +477,15 @@ def test_action_log_prob_gradient_against_differences():
         within(dx[ok, j], ((f(up) - f(dn)) / (2 * h))[ok], 40 * U * 8 / h + 4 * h * h, "dlogits")
 
 
-def test_action_log_prob_backward_keeps_its_own_mask():
-    """The environment's mask buffer is overwritten before the backward pass."""
+def test_action_log_prob_backward_keeps_its_own_mask_and_actions():
+    """The environment's mask and the collector's actions are overwritten before the backward pass."""
     x = torch.randn(4, 300, generator=gen(1), device="cuda", requires_grad=True)
     m = legal_mask(4, 300, 0.2, 5).to(torch.uint8)
     a = m.argmax(1).to(torch.int32)
     (want,) = torch.autograd.grad(P.action_log_prob(x, m, a)[0].sum(), x)
     lp, _ = P.action_log_prob(x, m, a)
     m.data.fill_(1)
+    a.data.fill_(-1)
     (got,) = torch.autograd.grad(lp.sum(), x)
     assert torch.equal(got, want)
 
