@@ -420,7 +420,9 @@ int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_
  * is drawn from max(p_i - q_i, 0) (from p_i where that leaves less than
  * 2^-40); after the last, from p at the place behind it.  Drawing takes the
  * least action whose running sum exceeds sample_u times the total.  What
- * comes out is distributed as the target's own play.  Computed in 64 bits.
+ * comes out is distributed as the target's own play.  The actions are those
+ * of 64-bit arithmetic; log-probabilities are rounded from it once, but those
+ * of kept drafts without a mask come from 32-bit sums.
  *
  * Outputs per game: `accepted` kept drafts; out_actions (drafts + 1): the
  * kept drafts, the drawn action, then -1; log_probs (drafts + 1): the

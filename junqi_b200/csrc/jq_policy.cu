@@ -555,6 +555,15 @@ struct Place {
         if (!y) return (double)u * p.z < ep;
         return q.state != Dist::SOME ? 0.0 < ep : __dmul_rn((double)u * q.weight(ya, table), p.z) < __dmul_rn(ep, q.z);
     }
+    // whether `kept` might turn with sums that are off by `eps`
+    __device__ __forceinline__ bool open(double eps, const double *table) const {
+        if (act < 0 || broken() || p.state != Dist::SOME) return false;
+        const double ep = p.weight(xa, table);
+        if (!y) return fabs((double)u * p.z - ep) <= eps * ep;
+        if (q.state != Dist::SOME) return false;
+        const double l = (double)u * q.weight(ya, table) * p.z, r = ep * q.z;
+        return fabs(l - r) <= eps * r && r > 0;
+    }
     // what is drawn from, times `scale`: max(p - q, 0) while `residual`, else p; ep, eq are exp(x - m) at j
     __device__ __forceinline__ bool has_residual() const { return drafted && (y ? q.state == Dist::SOME : act >= 0); }
     __device__ __forceinline__ double scale(bool residual) const { return residual && y ? p.z * q.z : p.z; }
@@ -748,7 +757,10 @@ __global__ void __launch_bounds__(ALONE ? 128 : 32 * PLACES, ALONE ? 8 : 3) veri
 // cluster: no row behind the first rejection is read (the next one is fetched
 // into L2 meanwhile).  A warp takes its own maximum and sum, and all tell all
 // others once per place and once for the draw; then the warp that has the
-// point goes on alone.
+// point goes on alone.  The sums that decide whether a draft is kept are in 32
+// bits first (a ninth of the instructions) and in 64 only where that could
+// turn the answer; what is drawn from is in 64 bits, but a row that is drawn
+// from alone needs no Z before.
 constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32, DENSE_CTAS = 8;
 
 // Every logit of x[0, n), by the warp: 8 bytes a load, the ends one by one.
@@ -776,18 +788,67 @@ __device__ __forceinline__ void dense_each(const T *x, int n, int lane, F &&f) {
     if (lane < rest) f(to_f(x[lane < head ? lane : lane + packs * VEC]));
 }
 
-// The largest of x[0, n), and the sum of exp(x - it), of a warp's chunk.
+// Running maximum and sum of exp(x - m) in 32 bits, of a warp's chunk.
+struct Sum {
+    float m, s;
+    __device__ __forceinline__ void raise(float c) {
+        if (c > m) s *= ex2((m - c) * LOG2E), m = c;
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const f2 (&x)[N]) {
+        float c = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c = fmaxf(c, fmaxf(parts(x[i]).x, parts(x[i]).y));
+        raise(c);
+        const f2 nm = both(-m), l = both(LOG2E);
+        f2 ss = both(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float2 w = parts((x[i] + nm) * l);
+            ss = ss + make_f2(ex2(w.x), ex2(w.y));
+        }
+        s += parts(ss).x + parts(ss).y;
+    }
+    __device__ __forceinline__ void join(float m2, float s2) {
+        const float top = fmaxf(m, m2);  // (of finite numbers, or +inf: then the sum is NaN)
+        s = (s == 0.f ? 0.f : s * ex2((m - top) * LOG2E)) + (s2 == 0.f ? 0.f : s2 * ex2((m2 - top) * LOG2E));
+        m = top;
+    }
+};
 template <typename T>
-__device__ __forceinline__ float dense_top(const T *x, int n, int lane) {
-    float top = -INFINITY;
-    dense_each(x, n, lane, [&](float v) { top = max_nan(top, v); });
-    return top;
+__device__ __forceinline__ Sum chunk_sum(const T *x, int n, int lane) {
+    constexpr int VEC = 8 / sizeof(T);
+    const int head = min(n, (int)((8 - ((uintptr_t)x & 7)) & 7) / (int)sizeof(T)), packs = (n - head) / VEC;
+    const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
+    Sum a{LOWEST, 0.f};
+    for (int k = lane; k < packs; k += 128) {
+        f2 v[2 * VEC];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            Pack<T, VEC> p;
+            const bool there = u == 0 || k + 32 * u < packs;
+            if (there) p = px[k + 32 * u];
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) v[u * VEC / 2 + i] = there ? to_f2(&p.v[2 * i]) : both(-INFINITY);
+        }
+        a.add(v);
+    }
+    const int rest = n - packs * VEC;  // before the first pack and behind the last
+    if (lane < rest) {
+        const f2 v[1] = {make_f2(to_f(x[lane < head ? lane : lane + packs * VEC]), -INFINITY)};
+        a.add(v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a.join(__shfl_xor_sync(ALL, a.m, o), __shfl_xor_sync(ALL, a.s, o));
+    return a;
 }
+
+// The same sum in 64 bits, m being given.
 template <typename T>
-__device__ __forceinline__ double dense_sum(const T *x, int n, int lane, const Dist &d, const double *table) {
+__device__ __forceinline__ double chunk_sum64(const T *x, int n, int lane, const Dist &d, const double *table) {
     double z = 0;
     if (d.state == Dist::SOME) dense_each(x, n, lane, [&](float v) { z += d.weight(v, table); });
-    return z;
+    return warp_sum(z);
 }
 
 template <typename T>
@@ -813,46 +874,49 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
         if (lane < 4 * ranks) cluster_store(&told[round][me][what], lane >> 2, what == 0 ? v0 : what == 1 ? v1 : what == 2 ? v2 : v3);
         cluster_sync();
     };
+    // how far a 32-bit sum may be off, relatively: 2^-22 for an exponential, its argument's three roundings of at most
+    // log2(n) <= 18 on average, one for each addition and 2^-22 for each time the maximum rose
+    const double eps = (3.0 * ((chunk + 31) / 32) + 160.0) / (1 << 24);
     for (int i = 0;; ++i) {
         Place<T> at(d, game, i, len);
+        bool exact = false;  // Z is in 64 bits
         {
-            float mx, my = -INFINITY;
-            double zx, zy = 0;
-            Dist own;
             if (i < len && 64 * lane < (c1 - c0) * (int)sizeof(T)) {  // the next place's chunk, on its way into L2
                 const int64_t by = (int64_t)c0 + 64 / (int)sizeof(T) * lane;
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(at.x + d.logits_place + by));
                 if (i + 1 < len && at.y) asm volatile("prefetch.global.L2 [%0];" ::"l"(at.y + d.draft_place + by));
             }
-            mx = dense_top(at.x + c0, c1 - c0, lane);
-            if (at.y) my = dense_top(at.y + c0, c1 - c0, lane);
+            const Sum sx = chunk_sum(at.x + c0, c1 - c0, lane);
+            Sum sy{LOWEST, 0.f};
+            if (at.y) sy = chunk_sum(at.y + c0, c1 - c0, lane);
             at.fetch();
-            mx = warp_max(mx), my = warp_max(my);
-            own.start(mx, true);
-            zx = dense_sum(at.x + c0, c1 - c0, lane, own, table);
-            if (at.y) {
-                own.start(my, true);
-                zy = dense_sum(at.y + c0, c1 - c0, lane, own, table);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) zx += __shfl_xor_sync(ALL, zx, o), zy += __shfl_xor_sync(ALL, zy, o);
-            tell((double)mx, zx, (double)my, zy);
-            const int k1 = lane + 32;
-            const float m0 = lane < warps ? (float)told[round][lane][0] : -INFINITY, m1 = k1 < warps ? (float)told[round][k1][0] : -INFINITY;
-            const float q0 = lane < warps ? (float)told[round][lane][2] : -INFINITY, q1 = k1 < warps ? (float)told[round][k1][2] : -INFINITY;
-            at.p.start(warp_max(max_nan(m0, m1)), true);
-            at.q.start(warp_max(max_nan(q0, q1)), at.y != nullptr);
-            double z = lane < warps ? told[round][lane][1] * at.p.weight(m0, table) : 0.0;
-            if (k1 < warps) z += told[round][k1][1] * at.p.weight(m1, table);
-            at.p.z = warp_sum(z);
-            if (at.y) {
-                z = lane < warps ? told[round][lane][3] * at.q.weight(q0, table) : 0.0;
-                if (k1 < warps) z += told[round][k1][3] * at.q.weight(q1, table);
-                at.q.z = warp_sum(z);
-            }
+            tell((double)sx.m, (double)sx.s, (double)sy.m, (double)sy.s);
+            // a chunk without a place above -inf has the sum 0, whatever its m; NaN or +inf make it NaN
+            auto total = [&](int what, Dist &dist, bool there) {
+                const int k1 = lane + 32;
+                const double s0 = lane < warps ? told[round][lane][what + 1] : 0.0, s1 = k1 < warps ? told[round][k1][what + 1] : 0.0;
+                const float m0 = s0 == 0.0 ? -INFINITY : s0 != s0 ? (float)s0 : (float)told[round][lane][what];
+                const float m1 = s1 == 0.0 ? -INFINITY : s1 != s1 ? (float)s1 : (float)told[round][k1][what];
+                dist.start(warp_max(max_nan(m0, m1)), there);
+                dist.z = warp_sum((s0 == 0.0 ? 0.0 : s0 * dist.weight(m0, table)) + (s1 == 0.0 ? 0.0 : s1 * dist.weight(m1, table)));
+            };
+            total(0, at.p, true);
+            total(2, at.q, at.y != nullptr);
             round ^= 1;
         }
-        if (at.kept(true, table)) {  // the same for the whole game: all its warps have the same numbers
+        // Z of both in 64 bits: where the 32-bit sums leave it open whether the draft is kept, and for what is drawn from both
+        auto make_exact = [&]() {
+            const double zx = chunk_sum64(at.x + c0, c1 - c0, lane, at.p, table);
+            const double zy = at.y ? chunk_sum64(at.y + c0, c1 - c0, lane, at.q, table) : 0.0;
+            tell(zx, zy, 0, 0);
+            at.p.z = warp_sum((lane < warps ? told[round][lane][0] : 0.0) + (lane + 32 < warps ? told[round][lane + 32][0] : 0.0));
+            at.q.z = warp_sum((lane < warps ? told[round][lane][1] : 0.0) + (lane + 32 < warps ? told[round][lane + 32][1] : 0.0));
+            round ^= 1;
+            exact = true;
+        };
+        // what all warps of the game have in the same numbers, they decide alike
+        if (at.open(4 * eps, table)) make_exact();
+        if (at.kept(true, table)) {
             if (me == 0 && lane == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
             continue;
         }
@@ -860,18 +924,25 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
         if (at.p.state == Dist::SOME && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
+            if (at.has_residual() && !exact) make_exact();
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
                 const bool residual = pass == 0;
                 auto weight = [&](int j) { return at.draw(j, residual, table); };
                 double part = 0;
+                if (residual) {
 #pragma unroll 4
-                for (int j = c0 + lane; j < c1; j += 32) part += weight(j);
-                tell(warp_sum(part), 0, 0, 0);
+                    for (int j = c0 + lane; j < c1; j += 32) part += weight(j);
+                    part = warp_sum(part);
+                } else {
+                    part = chunk_sum64(at.x + c0, c1 - c0, lane, at.p, table);
+                }
+                tell(part, 0, 0, 0);
                 // the first chunk whose running sum is above the point; with none, the last that has weight
                 const int per = (warps + 31) / 32, k0 = lane * per, k1 = k0 + 1;
                 const double t0 = k0 < warps ? told[round][k0][0] : 0.0, t1 = per > 1 && k1 < warps ? told[round][k1][0] : 0.0;
                 round ^= 1;
                 const double above = warp_scan(t0 + t1, lane), total = __shfl_sync(ALL, above, 31);
+                if (!exact && !residual) at.p.z = total;  // exp(x - m), summed up in 64 bits
                 if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
                 const double target = r * total, up = __shfl_up_sync(ALL, above, 1), before = lane ? up : 0.0;
                 unsigned cross = __ballot_sync(ALL, t0 + t1 > 0 && above > target), some = __ballot_sync(ALL, t0 + t1 > 0);
