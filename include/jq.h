@@ -375,7 +375,8 @@ enum { JQ_F32 = 0, JQ_F16 = 1, JQ_BF16 = 2 };
  * bias (either may be NULL: 1 and 0).  x, y are `dtype`, weight and bias
  * `wdtype` (JQ_F32 or `dtype`); statistics are 32-bit.  d_stats (rows x 3
  * floats: mean, what its rounding left, 1 / sqrt(var + eps)) is what the
- * backward pass reads, NULL when there will be none.  rows >= 1, dim >= 1. */
+ * backward pass reads, NULL when there will be none.  1 <= rows < 2^31,
+ * 1 <= dim <= 2^30. */
 int jq_layer_norm(const void *d_x, int64_t x_stride, const void *d_weight, const void *d_bias, int64_t rows,
                   int32_t dim, int32_t dtype, int32_t wdtype, float eps, void *d_y, float *d_stats, void *stream);
 

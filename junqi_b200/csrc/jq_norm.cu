@@ -679,7 +679,7 @@ static int norm_check(const void *x, int64_t x_stride, int64_t rows, int32_t dim
     if (!known_dtype(dtype)) return fail(JQ_ERR_ARG, "layer norm: unknown dtype");
     if (wdtype != JQ_F32 && wdtype != dtype) return fail(JQ_ERR_ARG, "layer norm: weights are float32 or of x's type");
     if (x_stride < 0) return fail(JQ_ERR_ARG, "layer norm: negative row stride");
-    if (rows > INT32_MAX) return fail(JQ_ERR_CAPACITY, "layer norm: more than 2^31 - 1 rows");
+    if (rows > INT32_MAX || dim > 1 << 30) return fail(JQ_ERR_CAPACITY, "layer norm: more than 2^31 - 1 rows or 2^30 places");
     return JQ_OK;
 }
 

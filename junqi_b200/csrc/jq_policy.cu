@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // sum exceeds r times the total.  The result is a whole number and borders
 // have to fall the same way for everybody, so everything is in 64 bits.
 //
-// The places of a game are worked on at the same time, up to 8 of them, and
+// The places of a game are worked on at the same time, up to 16 of them, and
 // the first that is not kept then draws: a game's chain is one place and one
 // draw, whatever its drafts.  That reads places behind the first rejection in
 // vain, but a game that goes place by place takes as long as its longest
@@ -488,8 +488,9 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // 1,024 of up to 8 drafts 54 us; place by place and a CTA per game these took
 // 89, 33 and 125.
 
+constexpr int VERIFY_WARPS = 36;  // of an SM, for the launch
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
-constexpr int PLACES = 8;      // of a game at the same time
+constexpr int PLACES = 16;     // of a game at the same time, at most
 
 struct VerifyArgs {
     jq_drafts d;
@@ -614,9 +615,9 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {
     return v;
 }
 
-// ALONE: no drafts, a game per warp.
+// ALONE: no drafts, a game per warp.  Bounds: 32 and 24 warps an SM by registers.
 template <typename T, bool ALONE>
-__global__ void __launch_bounds__(ALONE ? 128 : 32 * PLACES, ALONE ? 8 : 3) verify_masked_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(ALONE ? 128 : 768, ALONE ? 8 : 1) verify_masked_kernel(const VerifyArgs a) {
     extern __shared__ __align__(16) char verify_smem[];
     __shared__ double table[EXP_STEPS];
     __shared__ int keeps[2][PLACES];
@@ -767,18 +768,14 @@ __global__ void __launch_bounds__(ALONE ? 128 : 32 * PLACES, ALONE ? 8 : 3) veri
 }
 
 // Without a mask: a cluster of CTAs per game, each warp a consecutive chunk of
-// every row.  Place by place, since a place is enough work for the whole
-// cluster: no row behind the first rejection is read (the next one is fetched
-// into L2 meanwhile).  A warp takes its own maximum and sum, and all tell all
-// others once per place and once for the draw; then the warp that has the
-// point goes on alone.  The sums that decide whether a draft is kept are in 32
-// bits first (a ninth of the instructions) and in 64 only where that could
-// turn the answer; what is drawn from is in 64 bits, but a row that is drawn
-// from alone needs no Z before.  86 us for 301 games of up to 5 drafts over
-// 16,641 bfloat16 (all sums in 64 bits: 113; a CTA per place: 149); an
-// exponential in 64 bits costs 36 instructions of a warp, 12 of them on the
-// 64-bit units.
+// every row.  A warp takes its own maximum and sum of eight places' rows, in 32
+// bits (a ninth of the instructions of 64), and all tell all others once; warp
+// w of each CTA then finds out about place w.  Where 32 bits leave it open
+// whether a draft is kept, and for what is drawn from two rows, the sums are
+// taken again in 64.  The draw is in 64 bits: weights of the chunks, told once,
+// and the warp that has the point goes on alone.
 constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32, DENSE_CTAS = 8;
+constexpr int DENSE_PLACES = DENSE_WARPS;  // of a round
 
 // Every logit of x[0, n), by the warp: 8 bytes a load, the ends one by one.
 template <typename T, typename F>
@@ -868,15 +865,24 @@ __device__ __forceinline__ double chunk_sum64(const T *x, int n, int lane, const
     return warp_sum(z);
 }
 
+struct DenseSmem {
+    double table[EXP_STEPS];
+    float4 sums[2][DENSE_PLACES][DENSE_CTAS * DENSE_WARPS];  // by every warp of the game: m, sum of the target, of the draft
+    double told[2][DENSE_CTAS * DENSE_WARPS][2];             // by every warp of the game, in 64 bits
+    Dist p[DENSE_PLACES], q[DENSE_PLACES];
+    int found[DENSE_PLACES];
+};
+
 template <typename T>
 __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const VerifyArgs a) {
-    __shared__ double table[EXP_STEPS];
-    __shared__ double told[2][DENSE_CTAS * DENSE_WARPS][4];  // by every warp of the game: m, Z of the target, m, Z of the draft
+    enum { KEPT, LEFT, OPEN };
+    __shared__ DenseSmem sm;
     const jq_drafts &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 31, n = d.actions;
+    const double *table = sm.table;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = d.actions;
     const int rank = (int)cluster_rank(), ranks = (int)cluster_size(), game = blockIdx.x / ranks;
-    const int warps = ranks * DENSE_WARPS, me = rank * DENSE_WARPS + (tid >> 5);
-    if (tid < EXP_STEPS) table[tid] = exp_table(tid);
+    const int warps = ranks * DENSE_WARPS, me = rank * DENSE_WARPS + warp;
+    if (tid < EXP_STEPS) sm.table[tid] = exp_table(tid);
     pdl_enter();
     cluster_sync();  // the game's CTAs have all started: their shared memory may be written
     int len = d.lengths ? d.lengths[game] : d.drafts;
@@ -884,58 +890,85 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
     int32_t *out = d.out_actions + (int64_t)game * (d.drafts + 1);
     float *out_lp = d.log_probs + (int64_t)game * (d.drafts + 1);
     const int chunk = (n + warps - 1) / warps, c0 = min(n, me * chunk), c1 = min(n, c0 + chunk);
-    int round = 0;
-    // four numbers of this warp to every CTA
-    auto tell = [&](double v0, double v1, double v2, double v3) {
-        const int what = lane & 3;
-        if (lane < 4 * ranks) cluster_store(&told[round][me][what], lane >> 2, what == 0 ? v0 : what == 1 ? v1 : what == 2 ? v2 : v3);
+    int turn = 0;
+    // two numbers of this warp to every CTA
+    auto tell = [&](double v0, double v1) {
+        if (lane < 2 * ranks) cluster_store(&sm.told[turn][me][lane & 1], lane >> 1, lane & 1 ? v1 : v0);
         cluster_sync();
+    };
+    auto told = [&](int what) {  // their sum
+        return warp_sum((lane < warps ? sm.told[turn][lane][what] : 0.0) + (lane + 32 < warps ? sm.told[turn][lane + 32][what] : 0.0));
     };
     // how far a 32-bit sum may be off, relatively: 2^-22 for an exponential, its argument's three roundings of at most
     // log2(n) <= 18 on average, one for each addition and 2^-22 for each time the maximum rose
     const double eps = (3.0 * ((chunk + 31) / 32) + 160.0) / (1 << 24);
-    for (int i = 0;; ++i) {
-        Place<T> at(d, game, i, len);
-        bool exact = false;  // Z is in 64 bits
-        {
-            if (i < len && 64 * lane < (c1 - c0) * (int)sizeof(T)) {  // the next place's chunk, on its way into L2
+    for (int base = 0, round = 0;; round ^= 1) {
+        const int places = min(DENSE_PLACES, len - base + 1);
+        for (int k = 0; k < places; ++k) {
+            const Place<T> at(d, game, base + k, len);
+            if (k + 1 < places && 64 * lane < (c1 - c0) * (int)sizeof(T)) {  // the next place's chunk, on its way into L2
                 const int64_t by = (int64_t)c0 + 64 / (int)sizeof(T) * lane;
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(at.x + d.logits_place + by));
-                if (i + 1 < len && at.y) asm volatile("prefetch.global.L2 [%0];" ::"l"(at.y + d.draft_place + by));
+                if (base + k + 1 < len && at.y) asm volatile("prefetch.global.L2 [%0];" ::"l"(at.y + d.draft_place + by));
             }
             const Sum sx = chunk_sum(at.x + c0, c1 - c0, lane);
             Sum sy{LOWEST, 0.f};
             if (at.y) sy = chunk_sum(at.y + c0, c1 - c0, lane);
-            at.fetch();
-            tell((double)sx.m, (double)sx.s, (double)sy.m, (double)sy.s);
-            // a chunk without a place above -inf has the sum 0, whatever its m; NaN or +inf make it NaN
-            auto total = [&](int what, Dist &dist, bool there) {
-                const int k1 = lane + 32;
-                const double s0 = lane < warps ? told[round][lane][what + 1] : 0.0, s1 = k1 < warps ? told[round][k1][what + 1] : 0.0;
-                const float m0 = s0 == 0.0 ? -INFINITY : s0 != s0 ? (float)s0 : (float)told[round][lane][what];
-                const float m1 = s1 == 0.0 ? -INFINITY : s1 != s1 ? (float)s1 : (float)told[round][k1][what];
-                dist.start(warp_max(max_nan(m0, m1)), there);
-                dist.z = warp_sum((s0 == 0.0 ? 0.0 : s0 * dist.weight(m0, table)) + (s1 == 0.0 ? 0.0 : s1 * dist.weight(m1, table)));
-            };
-            total(0, at.p, true);
-            total(2, at.q, at.y != nullptr);
-            round ^= 1;
+            if (lane < ranks) cluster_store4(&sm.sums[round][k][me], lane, make_float4(sx.m, sx.s, sy.m, sy.s));
         }
-        // Z of both in 64 bits: where the 32-bit sums leave it open whether the draft is kept, and for what is drawn from both
+        cluster_sync();
+        if (warp < places) {
+            Place<T> at(d, game, base + warp, len);
+            at.fetch();
+            const float4 none = make_float4(0, 0, 0, 0);
+            const float4 s0 = lane < warps ? sm.sums[round][warp][lane] : none, s1 = lane + 32 < warps ? sm.sums[round][warp][lane + 32] : none;
+            // a chunk without a place above -inf has the sum 0, whatever its m; NaN or +inf make it NaN
+            auto total = [&](float m0, float v0, float m1, float v1, Dist &dist, bool there) {
+                m0 = v0 == 0.f ? -INFINITY : v0 != v0 ? v0 : m0;
+                m1 = v1 == 0.f ? -INFINITY : v1 != v1 ? v1 : m1;
+                dist.start(warp_max(max_nan(m0, m1)), there);
+                dist.z = warp_sum((v0 == 0.f ? 0.0 : v0 * dist.weight(m0, table)) + (v1 == 0.f ? 0.0 : v1 * dist.weight(m1, table)));
+            };
+            total(s0.x, s0.y, s1.x, s1.y, at.p, true);
+            total(s0.z, s0.w, s1.z, s1.w, at.q, at.y != nullptr);
+            const int found = at.open(4 * eps, table) ? OPEN : at.kept(true, table) ? KEPT : LEFT;
+            if (lane == 0) sm.p[warp] = at.p, sm.q[warp] = at.q, sm.found[warp] = found;
+        }
+        __syncthreads();
+        // what all CTAs of the game have in the same numbers, they decide alike
+        int first = places;
+        for (int k = places - 1; k >= 0; --k)
+            if (sm.found[k] != KEPT) first = k;
+        if (rank == 0 && warp < first && lane == 0) {
+            Place<T> at(d, game, base + warp, len);
+            at.p = sm.p[warp];
+            out[base + warp] = at.act, out_lp[base + warp] = at.log_prob(at.act);
+        }
+        if (first == places) {  // (the place behind the last draft is never kept)
+            base += places;
+            __syncthreads();
+            continue;
+        }
+        const int i = base + first;
+        Place<T> at(d, game, i, len);
+        at.p = sm.p[first], at.q = sm.q[first];
+        bool exact = false;  // Z is in 64 bits
         auto make_exact = [&]() {
             const double zx = chunk_sum64(at.x + c0, c1 - c0, lane, at.p, table);
-            const double zy = at.y ? chunk_sum64(at.y + c0, c1 - c0, lane, at.q, table) : 0.0;
-            tell(zx, zy, 0, 0);
-            at.p.z = warp_sum((lane < warps ? told[round][lane][0] : 0.0) + (lane + 32 < warps ? told[round][lane + 32][0] : 0.0));
-            at.q.z = warp_sum((lane < warps ? told[round][lane][1] : 0.0) + (lane + 32 < warps ? told[round][lane + 32][1] : 0.0));
-            round ^= 1;
+            tell(zx, at.y ? chunk_sum64(at.y + c0, c1 - c0, lane, at.q, table) : 0.0);
+            at.p.z = told(0), at.q.z = told(1);
+            turn ^= 1;
             exact = true;
         };
-        // what all warps of the game have in the same numbers, they decide alike
-        if (at.open(4 * eps, table)) make_exact();
-        if (at.kept(true, table)) {
-            if (me == 0 && lane == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
-            continue;
+        if (sm.found[first] == OPEN) {
+            at.fetch();
+            make_exact();
+            if (at.kept(true, table)) {
+                if (me == 0 && lane == 0) out[i] = at.act, out_lp[i] = at.log_prob(at.act);
+                base = i + 1;
+                __syncthreads();
+                continue;
+            }
         }
         int next = -1, who = 0;  // who: the warp whose chunk has the point
         if (at.p.state == Dist::SOME && !at.broken()) {
@@ -953,11 +986,11 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
                 } else {
                     part = chunk_sum64(at.x + c0, c1 - c0, lane, at.p, table);
                 }
-                tell(part, 0, 0, 0);
+                tell(part, 0);
                 // the first chunk whose running sum is above the point; with none, the last that has weight
                 const int per = (warps + 31) / 32, k0 = lane * per, k1 = k0 + 1;
-                const double t0 = k0 < warps ? told[round][k0][0] : 0.0, t1 = per > 1 && k1 < warps ? told[round][k1][0] : 0.0;
-                round ^= 1;
+                const double t0 = k0 < warps ? sm.told[turn][k0][0] : 0.0, t1 = per > 1 && k1 < warps ? sm.told[turn][k1][0] : 0.0;
+                turn ^= 1;
                 const double above = warp_scan(t0 + t1, lane), total = __shfl_sync(ALL, above, 31);
                 if (!exact && !residual) at.p.z = total;  // exp(x - m), summed up in 64 bits
                 if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
@@ -1069,10 +1102,13 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
         CU(launch_pdl(verify_masked_kernel<T, true>, (unsigned)((d.games + warps - 1) / warps), 32 * warps, warps * a.share, s, a));
         return JQ_OK;
     }
-    int sms, rc = device_sms(sms), warps = d.drafts + 1 < PLACES ? d.drafts + 1 : PLACES;
+    int sms, rc = device_sms(sms);
     if (rc) return rc;
-    // as many places side by side as keep all games on the SMs at once (24 warps each), since the longest chain counts
-    while (warps > 2 && (int64_t)d.games * warps > 24 * (int64_t)sms) --warps;
+    // places side by side: as few rounds as there are warps for, about WAVES times what the SMs hold (24 each), and no more
+    // places than those rounds need
+    const int places = d.drafts + 1;
+    int rounds = (places + PLACES - 1) / PLACES, warps = (places + rounds - 1) / rounds;
+    while (warps > 2 && (int64_t)d.games * warps > VERIFY_WARPS * (int64_t)sms) ++rounds, warps = (places + rounds - 1) / rounds;
     while (warps > 1 && warps * a.share > 200 * 1024) --warps;
     if (warps * a.share > 40 * 1024) CU(allow_smem(verify_masked_kernel<T, false>, 210 * 1024, raised[0]));
     CU(launch_pdl(verify_masked_kernel<T, false>, (unsigned)d.games, 32 * warps, warps * a.share, s, a));

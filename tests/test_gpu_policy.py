@@ -637,6 +637,36 @@ def test_verify_drafts_bad_drafts_and_lengths():
         check_verify(x, a, au, su, None, mask, lengths)
 
 
+@pytest.mark.parametrize("masked", [True, False])
+@pytest.mark.parametrize("n", [50, 16641])
+@pytest.mark.parametrize("scored", [True, False])
+def test_verify_drafts_at_the_borders(masked, n, scored):
+    """accept_u at p / q itself and the 32-bit numbers next to it (at most 2^-24 away, relatively), and sample_u next
+    to a border between two actions: the choices are those of 64 bits."""
+    games, d = 60, 3
+    x, a, au, su, y, mask = drafted(games, d, n, torch.float32, 11 + n, 0.2 if masked else None)
+    legal = torch.ones(x.shape, dtype=torch.bool, device="cuda") if mask is None else mask
+
+    def dist(t, m):
+        t = t.double().masked_fill(~m, -torch.inf)
+        return (t - t.amax(-1, keepdim=True).clamp(min=-1e9)).softmax(-1).nan_to_num()
+
+    p, q = dist(x, legal), dist(y, legal[:, :d])
+    at = a.long().clamp(min=0)[..., None]
+    ratio = p[:, :d].gather(2, at)[..., 0] / (q.gather(2, at)[..., 0] if scored else 1.0)
+    border = ratio.clamp(max=1 - 2.0 ** -24).nan_to_num().float()
+    step = torch.arange(games, device="cuda")[:, None] % 3 - 1
+    au = torch.where(step == 0, border, torch.nextafter(border, step.float().expand(games, d) * 10)).clamp(0, 1 - 2.0 ** -24)
+    w = p[:, d]
+    run = w.cumsum(1)
+    j = torch.multinomial(w + 1e-12, 1, generator=gen(4))
+    su = run.gather(1, j)[:, 0].clamp(max=1 - 2.0 ** -24).float()
+    for lengths in (None, torch.zeros(games, dtype=torch.int32, device="cuda")):
+        v = P.verify_drafts(x, a, au, su, draft_logits=y if scored else None, mask=mask, lengths=lengths)
+        acc, out, _ = plain_verify(x, a, au, su, y if scored else None, mask, lengths)
+        assert np.array_equal(v.accepted.cpu().numpy(), acc) and np.array_equal(v.actions.cpu().numpy(), out)
+
+
 def test_verify_drafts_extreme_random_numbers():
     """0, the largest number below 1, and, though not allowed, 1 and more, negative ones and NaN."""
     x, a, au, su, y, mask = drafted(40, 3, 200, torch.float32, 5, 0.2)
@@ -725,6 +755,25 @@ def test_verified_play_is_distributed_as_the_target():
     assert ((share - p).abs() <= 4 / k).all(), (share, p)
 
 
+def test_verify_drafts_beyond_32_bit_offsets():
+    games, d, n = 33_000, 3, 16641
+    x, a, au, su, y, mask = drafted(6, d, n, torch.bfloat16, 3, 0.01)
+    big = torch.zeros(games, d + 1, n, dtype=torch.bfloat16, device="cuda")
+    big[-6:] = x
+    legal = torch.zeros(games, d + 1, n, dtype=torch.uint8, device="cuda")
+    legal[-6:] = mask
+    drafts = torch.zeros(games, d, dtype=torch.int32, device="cuda")
+    drafts[-6:] = a
+    u, r = torch.full((games, d), 0.5, device="cuda"), torch.full((games,), 0.5, device="cuda")
+    u[-6:], r[-6:] = au, su
+    for m in (legal, None):
+        v = P.verify_drafts(big, drafts, u, r, mask=m)
+        w = check_verify(x, a, au, su, None, None if m is None else mask)
+        assert torch.equal(v.accepted[-6:], w.accepted) and torch.equal(v.actions[-6:], w.actions)
+        if m is not None:  # nothing legal anywhere else
+            assert not v.accepted[:-6].any() and (v.actions[:-6] == -1).all() and not v.log_probs[:-6].any()
+
+
 # -- streams and graphs ------------------------------------------------------------------
 
 def test_other_streams():
@@ -748,6 +797,39 @@ def test_other_streams():
     torch.cuda.current_stream().wait_stream(side)
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+def test_two_threads_at_once():
+    """Calls of two threads, each on a stream of its own, forward and backward."""
+    import threading
+    x = torch.randn(200, 700, generator=gen(1), device="cuda")
+    m = legal_mask(200, 700, 0.1, 2)
+    u = torch.rand(200, generator=gen(3), device="cuda")
+
+    def work():
+        leaf = x.clone().requires_grad_(True)
+        y = P.layer_norm(leaf)
+        a, _ = P.sample_actions(y, m, u)
+        lp, ent = P.action_log_prob(y, m, a)
+        return a, lp.detach(), torch.autograd.grad(lp.sum() + ent.sum(), leaf)[0]
+
+    want = work()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = work()
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(1 for g, w in zip(got, want) if not torch.equal(g, w))
+
+    threads = [threading.Thread(target=run) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
 
 
 def test_graphs_replay_on_new_inputs():

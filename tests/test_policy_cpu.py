@@ -109,6 +109,9 @@ def test_entry_points_refuse_before_they_launch():
                     (dict(y=None), "output"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps")):
         st, msg = ln(**k)
         assert st == 1 and text in msg, (k, st, msg)
+    for k in (dict(rows=2 ** 31), dict(dim=2 ** 30 + 1)):
+        st, msg = ln(**k)
+        assert st == 4 and "more than" in msg, (k, st, msg)
     lp = lambda **k: _status("jq_action_log_prob", *({**dict(x=p, xs=8, dt=0, m=p, ms=8, a=p, rows=4, n=8, lp=p, e=p,  # noqa: E731
                                                              st=p, bits=p, s=None), **k}).values())
     for k, want, text in ((dict(x=None), 1, "at least one row"), (dict(rows=0), 1, "at least"), (dict(n=0), 1, "at least"),
