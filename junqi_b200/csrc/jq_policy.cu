@@ -767,13 +767,14 @@ __global__ void __launch_bounds__(ALONE ? 128 : 768, ALONE ? 8 : 1) verify_maske
     }
 }
 
-// Without a mask: a cluster of CTAs per game, each warp a consecutive chunk of
-// every row.  A warp takes its own maximum and sum of eight places' rows, in 32
-// bits (a ninth of the instructions of 64), and all tell all others once; warp
-// w of each CTA then finds out about place w.  Where 32 bits leave it open
-// whether a draft is kept, and for what is drawn from two rows, the sums are
-// taken again in 64.  The draw is in 64 bits: weights of the chunks, told once,
-// and the warp that has the point goes on alone.
+// Without a mask: a cluster of CTAs per game, each a consecutive slice of every
+// row.  For eight places at a time a warp takes the maximum and sum of one
+// place's rows over the slice, in 32 bits (a ninth of the instructions of 64),
+// and all tell all others once; warp w of each CTA then finds out about place
+// w.  Where 32 bits leave it open whether a draft is kept, and for what is drawn
+// from two rows, the sums are taken again in 64, every warp a chunk of the row.
+// The draw is in 64 bits: weights of the chunks, told once, and the warp that
+// has the point goes on alone.
 constexpr int DENSE_THREADS = 256, DENSE_WARPS = DENSE_THREADS / 32, DENSE_CTAS = 8;
 constexpr int DENSE_PLACES = DENSE_WARPS;  // of a round
 
@@ -802,7 +803,7 @@ __device__ __forceinline__ void dense_each(const T *x, int n, int lane, F &&f) {
     if (lane < rest) f(to_f(x[lane < head ? lane : lane + packs * VEC]));
 }
 
-// Running maximum and sum of exp(x - m) in 32 bits, of a warp's chunk.
+// Running maximum and sum of exp(x - m) in 32 bits, of a warp's part of a row.
 struct Sum {
     float m, s;
     __device__ __forceinline__ void raise(float c) {
@@ -835,6 +836,8 @@ __device__ __forceinline__ Sum chunk_sum(const T *x, int n, int lane) {
     const int head = min(n, (int)((8 - ((uintptr_t)x & 7)) & 7) / (int)sizeof(T)), packs = (n - head) / VEC;
     const Pack<T, VEC> *px = (const Pack<T, VEC> *)(x + head);
     Sum a{LOWEST, 0.f};
+    const int rest = n - packs * VEC;  // before the first pack and behind the last
+    const float end = lane < rest ? to_f(x[lane < head ? lane : lane + packs * VEC]) : -INFINITY;
     for (int k = lane; k < packs; k += 128) {
         f2 v[2 * VEC];
 #pragma unroll
@@ -847,11 +850,8 @@ __device__ __forceinline__ Sum chunk_sum(const T *x, int n, int lane) {
         }
         a.add(v);
     }
-    const int rest = n - packs * VEC;  // before the first pack and behind the last
-    if (lane < rest) {
-        const f2 v[1] = {make_f2(to_f(x[lane < head ? lane : lane + packs * VEC]), -INFINITY)};
-        a.add(v);
-    }
+    const f2 v[1] = {make_f2(end, -INFINITY)};
+    a.add(v);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a.join(__shfl_xor_sync(ALL, a.m, o), __shfl_xor_sync(ALL, a.s, o));
     return a;
@@ -867,7 +867,7 @@ __device__ __forceinline__ double chunk_sum64(const T *x, int n, int lane, const
 
 struct DenseSmem {
     double table[EXP_STEPS];
-    float4 sums[2][DENSE_PLACES][DENSE_CTAS * DENSE_WARPS];  // by every warp of the game: m, sum of the target, of the draft
+    float4 sums[2][DENSE_PLACES][DENSE_CTAS * DENSE_WARPS];  // by every warp at work on the place: m, sum of the target, of the draft
     double told[2][DENSE_CTAS * DENSE_WARPS][2];             // by every warp of the game, in 64 bits
     Dist p[DENSE_PLACES], q[DENSE_PLACES];
     int found[DENSE_PLACES];
@@ -899,29 +899,30 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
     auto told = [&](int what) {  // their sum
         return warp_sum((lane < warps ? sm.told[turn][lane][what] : 0.0) + (lane + 32 < warps ? sm.told[turn][lane + 32][what] : 0.0));
     };
-    // how far a 32-bit sum may be off, relatively: 2^-22 for an exponential, its argument's three roundings of at most
-    // log2(n) <= 18 on average, one for each addition and 2^-22 for each time the maximum rose
-    const double eps = (3.0 * ((chunk + 31) / 32) + 160.0) / (1 << 24);
+    const int slice = (n + ranks - 1) / ranks, s0 = min(n, rank * slice), s1 = min(n, s0 + slice);
     for (int base = 0, round = 0;; round ^= 1) {
         const int places = min(DENSE_PLACES, len - base + 1);
-        for (int k = 0; k < places; ++k) {
+        // a place of this CTA's slice is one warp's, or several warps'
+        const int split = DENSE_WARPS / places, k = warp / split, part_of = warp % split, share = (slice + split - 1) / split;
+        // how far a 32-bit sum may be off, relatively: 2^-22 for an exponential, its argument's three roundings of at most
+        // log2(n) <= 18 on average, one for each addition and 2^-22 for each time the maximum rose
+        const double eps = (3.0 * ((share + 31) / 32) + 160.0) / (1 << 24);
+        if (k < places) {
             const Place<T> at(d, game, base + k, len);
-            if (k + 1 < places && 64 * lane < (c1 - c0) * (int)sizeof(T)) {  // the next place's chunk, on its way into L2
-                const int64_t by = (int64_t)c0 + 64 / (int)sizeof(T) * lane;
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(at.x + d.logits_place + by));
-                if (base + k + 1 < len && at.y) asm volatile("prefetch.global.L2 [%0];" ::"l"(at.y + d.draft_place + by));
-            }
-            const Sum sx = chunk_sum(at.x + c0, c1 - c0, lane);
+            const int b0 = min(s1, s0 + part_of * share), b1 = min(s1, b0 + share);
+            const Sum sx = chunk_sum(at.x + b0, b1 - b0, lane);
             Sum sy{LOWEST, 0.f};
-            if (at.y) sy = chunk_sum(at.y + c0, c1 - c0, lane);
-            if (lane < ranks) cluster_store4(&sm.sums[round][k][me], lane, make_float4(sx.m, sx.s, sy.m, sy.s));
+            if (at.y) sy = chunk_sum(at.y + b0, b1 - b0, lane);
+            if (lane < ranks) cluster_store4(&sm.sums[round][k][rank * split + part_of], lane, make_float4(sx.m, sx.s, sy.m, sy.s));
         }
         cluster_sync();
         if (warp < places) {
             Place<T> at(d, game, base + warp, len);
             at.fetch();
             const float4 none = make_float4(0, 0, 0, 0);
-            const float4 s0 = lane < warps ? sm.sums[round][warp][lane] : none, s1 = lane + 32 < warps ? sm.sums[round][warp][lane + 32] : none;
+            const int parts = ranks * split;
+            const float4 t0 = lane < parts ? sm.sums[round][warp][lane] : none,
+                         t1 = lane + 32 < parts ? sm.sums[round][warp][lane + 32] : none;
             // a chunk without a place above -inf has the sum 0, whatever its m; NaN or +inf make it NaN
             auto total = [&](float m0, float v0, float m1, float v1, Dist &dist, bool there) {
                 m0 = v0 == 0.f ? -INFINITY : v0 != v0 ? v0 : m0;
@@ -929,8 +930,8 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
                 dist.start(warp_max(max_nan(m0, m1)), there);
                 dist.z = warp_sum((v0 == 0.f ? 0.0 : v0 * dist.weight(m0, table)) + (v1 == 0.f ? 0.0 : v1 * dist.weight(m1, table)));
             };
-            total(s0.x, s0.y, s1.x, s1.y, at.p, true);
-            total(s0.z, s0.w, s1.z, s1.w, at.q, at.y != nullptr);
+            total(t0.x, t0.y, t1.x, t1.y, at.p, true);
+            total(t0.z, t0.w, t1.z, t1.w, at.q, at.y != nullptr);
             const int found = at.open(4 * eps, table) ? OPEN : at.kept(true, table) ? KEPT : LEFT;
             if (lane == 0) sm.p[warp] = at.p, sm.q[warp] = at.q, sm.found[warp] = found;
         }
@@ -1001,26 +1002,38 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
                 who = __shfl_sync(ALL, second ? k1 : k0, owner);
                 double below = __shfl_sync(ALL, second ? before + t0 : before, owner);
                 if (who != me) return;
-                // of the chunk a lane has consecutive places, of those 32 at a time one each
-                const int share = (c1 - c0 + 31) / 32;
-                int f = min(c1, c0 + lane * share);
-                const int g = min(c1, f + share);
-                part = 0;
-#pragma unroll 4
-                for (int j = f; j < g; ++j) part += weight(j);
-                const double sum = warp_scan(part, lane), lower = __shfl_up_sync(ALL, sum, 1);
-                cross = __ballot_sync(ALL, part > 0 && below + sum > target), some = __ballot_sync(ALL, part > 0);
-                owner = cross ? __ffs(cross) - 1 : 31 - __clz(some);
-                below += __shfl_sync(ALL, lane ? lower : 0.0, owner);
-                f = __shfl_sync(ALL, f, owner);
-                const int end = __shfl_sync(ALL, g, owner);
-                for (; f < end; f += 32) {
-                    const double w = f + lane < end ? weight(f + lane) : 0.0, run = warp_scan(w, lane);
-                    cross = __ballot_sync(ALL, w > 0 && below + run > target), some = __ballot_sync(ALL, w > 0);
-                    if (some) next = f + (cross ? __ffs(cross) - 1 : 31 - __clz(some));
-                    if (cross) break;
-                    below += __shfl_sync(ALL, run, 31);
+                // 256 places at a time, eight consecutive ones a lane; whether the point is in them, or the last weight may be
+                constexpr int STEP = 8;
+                auto look = [&](int f, bool last) {
+                    double w[STEP], s = 0;
+#pragma unroll
+                    for (int k = 0; k < STEP; ++k) {
+                        const int j = f + STEP * lane + k;
+                        w[k] = j < c1 ? weight(j) : 0.0;
+                        s += w[k];
+                    }
+                    const double sum = warp_scan(s, lane), up = __shfl_up_sync(ALL, sum, 1);
+                    cross = __ballot_sync(ALL, !last && s > 0 && below + sum > target), some = __ballot_sync(ALL, s > 0);
+                    if (cross || last) {
+                        double run = below + (lane ? up : 0.0);
+                        bool crossed = false;
+                        int at_j = -1;
+#pragma unroll
+                        for (int k = 0; k < STEP; ++k) {
+                            run += w[k];
+                            if (w[k] > 0 && !crossed) at_j = f + STEP * lane + k, crossed = !last && run > target;
+                        }
+                        next = __shfl_sync(ALL, at_j, cross ? __ffs(cross) - 1 : 31 - __clz(some));
+                    }
+                    below += __shfl_sync(ALL, sum, 31);
+                };
+                int held = c0;
+                cross = 0;
+                for (int f = c0; f < c1 && !cross; f += 32 * STEP) {
+                    look(f, false);
+                    if (some) held = f;
                 }
+                if (!cross) look(held, true);  // the point is at the end of the chunk's sum: its last place with weight
                 break;
             }
         }
