@@ -111,18 +111,13 @@ struct Legal {
         blocks = pack_mask((uint16_t *)bits, found, most, mask, places, lane);
         __syncwarp();
     }
-    // The places in order, as far as there are at most LIST, and their number; [w0, w1): this lane's share of the words.
-    __device__ __forceinline__ int list(int *to, int lane, int &w0, int &w1) const {
-        const int share = (words + 31) >> 5;
-        w0 = min(words, lane * share), w1 = min(words, w0 + share);
+    // The places in order, as far as there are at most LIST, and their number.
+    __device__ __forceinline__ int list(int *to, int lane) const {
         // this lane's: of its share of the blocks that have some, or of the words
         const bool few = blocks <= most;
-        const int per = (blocks + 31) >> 5, e0 = min(blocks, lane * per), e1 = min(blocks, e0 + per);
+        const int share = ((few ? blocks : words) + 31) >> 5, e0 = lane * share, e1 = min(few ? blocks : words, e0 + share);
         int before = 0;
-        if (few)
-            for (int e = e0; e < e1; ++e) before += __popc(found[e] & 0xffff);
-        else
-            for (int w = w0; w < w1; ++w) before += __popc(bits[w]);
+        for (int e = e0; e < e1; ++e) before += __popc(few ? found[e] & 0xffff : bits[e]);
         const int own = before;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -136,6 +131,31 @@ struct Legal {
                 const int j0 = (int)(found[e] >> 16) * 16 - skip;
                 for (uint32_t b = found[e] & 0xffff; b; b &= b - 1) to[before++] = j0 + __ffs(b) - 1;
             }
+        __syncwarp();
+        return count;
+    }
+    // The next ones in order from word w on, whole words of them, at most LIST places, and their number; w: behind them.
+    // (With more than LIST legal actions the list holds a part of them at a time, for the maximum, the sum and the draw
+    // again: 1,000 games of up to 8 drafts of 16,641 bfloat16 with up to 512 take 150 us; a lane per place of every word of
+    // the mask, which kept no list, took 1,040.)
+    __device__ __forceinline__ int part(int *to, int lane, int &w) const {
+        __syncwarp();  // the last part has been read
+        int count = 0, took = 32;
+        while (took == 32) {
+            uint32_t b = w + lane < words ? bits[w + lane] : 0;
+            int upto = __popc(b);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(ALL, upto, o);
+                if (lane >= o) upto += u;
+            }
+            const bool fits = w + lane < words && count + upto <= LIST;
+            took = __popc(__ballot_sync(ALL, fits));  // (ten words or more, as far as there are any)
+            if (fits)
+                for (int k = count + upto - __popc(b); b; b &= b - 1) to[k++] = 32 * (w + lane) + __ffs(b) - 1 - skip;
+            if (took) count += __shfl_sync(ALL, upto, took - 1);
+            w += took;
+        }
         __syncwarp();
         return count;
     }
@@ -484,9 +504,9 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // what bounds it is the mask's bytes (with many games) or the chain of some
 // thousand cycles (with few).  Without a mask the bound is the exponentials in
 // 64 bits (verify_dense_kernel).  Measured: 4,096 samples of 16,641 float32 with
-// up to 80 legal actions 20 us (69 MB, 3.4 TB/s), 8 games of 4 drafts 8.5 us,
-// 1,024 of up to 8 drafts 54 us; place by place and a CTA per game these took
-// 89, 33 and 125.
+// up to 80 legal actions 20 us (69 MB, 3.4 TB/s), 8 games of 4 drafts 8.9 us,
+// 1,024 of up to 8 drafts 43 us; place by place and a CTA per game these took
+// 89, 33 and 125.  301 games of 5 drafts without a mask 75 us.
 
 constexpr int VERIFY_WARPS = 36;  // of an SM, for the launch
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
@@ -646,78 +666,76 @@ __global__ void __launch_bounds__(ALONE ? 128 : 768, ALONE ? 8 : 1) verify_maske
         bool kept = false;
         Place<T> at(d, game, active ? i : len, len);
         if (ALONE) at.y = nullptr, at.act = -1, at.drafted = false;
-        int count = 0, lo = 0, hi = 0, w0 = 0, w1 = 0;
-        // this lane's legal actions, consecutive ones, with their exp(x - m): of the list, or of the packed mask
-        auto each = [&](auto &&f) {
-            if (count <= LIST) {
-                for (int k = lo; k < hi; ++k) f(list[k], ep[k], at.y ? eq[k] : 0.0);
-            } else {
-                for (int w = w0; w < w1; ++w)
-                    for (uint32_t b = legal.bits[w]; b; b &= b - 1) {
-                        const int j = 32 * w + __ffs(b) - 1 - legal.skip;
-                        f(j, at.p.weight(to_f(at.x[j]), table), at.y ? at.q.weight(to_f(at.y[j]), table) : 0.0);
+        int count = 0, w = 0;  // on the list; the mask's word behind it
+        bool whole = true;     // the list has all legal actions, and stays; else it holds a part of them at a time
+        float mx = -INFINITY, my = -INFINITY;
+        double zx = 0, zy = 0;
+        auto logits = [&]() {  // the list's, four scattered logits of each in flight
+            for (int k0 = lane; k0 < count; k0 += 128) {
+                float vx[4], vy[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k0 + 32 * i < count) {
+                        const int j = list[k0 + 32 * i];
+                        vx[i] = to_f(at.x[j]);
+                        if (at.y) vy[i] = to_f(at.y[j]);
                     }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k0 + 32 * i < count) {
+                        mx = max_nan(mx, vx[i]);
+                        ep[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vx[i]));
+                        if (at.y) {
+                            my = max_nan(my, vy[i]);
+                            eq[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vy[i]));
+                        }
+                    }
+            }
+        };
+        auto weights = [&]() {  // exp(x - m) in the logits' place
+#pragma unroll 2
+            for (int k = lane; k < count; k += 32) {
+                const double e = at.p.weight(__int_as_float(__double2loint(ep[k])), table);
+                ep[k] = e, zx += e;
+                if (at.y) {
+                    const double g = at.q.weight(__int_as_float(__double2loint(eq[k])), table);
+                    eq[k] = g, zy += g;
+                }
+            }
+            __syncwarp();  // other lanes read them
+        };
+        auto next_part = [&]() {
+            count = legal.part(list, lane, w);
+            if constexpr (ALONE) {
+                logits();
+            } else {
+#pragma unroll 1
+                for (int k = lane; k < count; k += 32) {  // one at a time, or the whole list's four lose registers
+                    const float vx = to_f(at.x[list[k]]), vy = at.y ? to_f(at.y[list[k]]) : -INFINITY;
+                    mx = max_nan(mx, vx), my = max_nan(my, vy);
+                    ep[k] = __hiloint2double(0, __float_as_int(vx));
+                    if (at.y) eq[k] = __hiloint2double(0, __float_as_int(vy));
+                }
             }
         };
         if (active) {
             legal.read(at.mask, n, lane);
             at.fetch();
-            count = legal.list(list, lane, w0, w1);
-            float mx = -INFINITY, my = -INFINITY;
-            double zx = 0, zy = 0;
-            if (count <= LIST) {
-                const int per = (count + 31) >> 5;
-                lo = min(count, lane * per), hi = min(count, lo + per);
-                for (int k0 = lane; k0 < count; k0 += 128) {  // four scattered logits of each in flight
-                    float vx[4], vy[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (k0 + 32 * i < count) {
-                            const int j = list[k0 + 32 * i];
-                            vx[i] = to_f(at.x[j]);
-                            if (at.y) vy[i] = to_f(at.y[j]);
-                        }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (k0 + 32 * i < count) {
-                            mx = max_nan(mx, vx[i]);
-                            ep[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vx[i]));
-                            if (at.y) {
-                                my = max_nan(my, vy[i]);
-                                eq[k0 + 32 * i] = __hiloint2double(0, __float_as_int(vy[i]));
-                            }
-                        }
-                }
-            } else {
-                for (int w = 0; w < legal.words; ++w)  // many: a lane per place
-                    if ((legal.bits[w] >> lane) & 1) {
-                        mx = max_nan(mx, to_f(at.x[32 * w + lane - legal.skip]));
-                        if (at.y) my = max_nan(my, to_f(at.y[32 * w + lane - legal.skip]));
-                    }
-            }
+            count = legal.list(list, lane);
+            whole = count <= LIST;
+            if (whole)
+                logits();
+            else
+                while (w < legal.words) next_part();
             at.p.start(warp_max(mx), true);
             at.q.start(warp_max(my), at.y != nullptr);
-            if (count <= LIST) {
-#pragma unroll 2
-                for (int k = lane; k < count; k += 32) {
-                    const double e = at.p.weight(__int_as_float(__double2loint(ep[k])), table);
-                    ep[k] = e, zx += e;
-                    if (at.y) {
-                        const double g = at.q.weight(__int_as_float(__double2loint(eq[k])), table);
-                        eq[k] = g, zy += g;
-                    }
-                }
-            } else {
-                for (int w = 0; w < legal.words; ++w)
-                    if ((legal.bits[w] >> lane) & 1) {
-                        zx += at.p.weight(to_f(at.x[32 * w + lane - legal.skip]), table);
-                        if (at.y) zy += at.q.weight(to_f(at.y[32 * w + lane - legal.skip]), table);
-                    }
-            }
+            if (whole)
+                weights();
+            else
+                for (w = 0; w < legal.words;) next_part(), weights();
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) zx += __shfl_xor_sync(ALL, zx, o), zy += __shfl_xor_sync(ALL, zy, o);
             at.p.z = zx, at.q.z = zy;
-            __syncwarp();  // the list's exponentials are read by other lanes
             kept = at.kept(at.act >= 0 && legal.has(at.act), table);
         }
         int first = ALONE ? 0 : warps;  // the first place of this round that is not kept
@@ -735,24 +753,42 @@ __global__ void __launch_bounds__(ALONE ? 128 : 768, ALONE ? 8 : 1) verify_maske
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
             auto draw = [&](bool residual) {  // false: nothing left to draw from
-                double part = 0;
-                each([&](int j, double p, double q) { part += at.draw(j, p, q, residual); });
-                const double above = warp_scan(part, lane), total = __shfl_sync(ALL, above, 31);
+                double part, above, total = 0, below = 0;
+                // this lane's actions are consecutive ones of the list: its weight, and with the lanes before
+                auto sum_up = [&]() {
+                    const int per = (count + 31) >> 5, lo = lane * per, hi = min(count, lo + per);
+                    part = 0;
+                    for (int k = lo; k < hi; ++k) part += at.draw(list[k], ep[k], at.y ? eq[k] : 0.0, residual);
+                    above = warp_scan(part, lane);
+                };
+                if (whole)
+                    sum_up(), total = __shfl_sync(ALL, above, 31);
+                else
+                    for (w = 0; w < legal.words; total += __shfl_sync(ALL, above, 31)) next_part(), weights(), sum_up();
                 if (residual && !(total > RESIDUAL_MIN * at.scale(true))) return false;
-                const double up = __shfl_up_sync(ALL, above, 1), below = lane ? up : 0.0, target = r * total;
-                // the first lane whose running sum is above the point; with none, the last that has weight
-                const unsigned cross = __ballot_sync(ALL, part > 0 && above > target), some = __ballot_sync(ALL, part > 0);
-                const int who = cross ? __ffs(cross) - 1 : 31 - __clz(some);
-                if (lane == who) {
-                    double run = below;
-                    bool crossed = false;
-                    each([&](int j, double p, double q) {
-                        const double w = at.draw(j, p, q, residual);
-                        run += w;
-                        if (w > 0 && !crossed) next = j, crossed = run > target;
-                    });
-                }
-                next = __shfl_sync(ALL, next, who);
+                const double target = r * total;
+                unsigned cross = 0;
+                w = 0;
+                do {
+                    if (!whole) next_part(), weights(), sum_up();
+                    // the first lane whose running sum is above the point; with none, the last that has weight
+                    const double up = __shfl_up_sync(ALL, above, 1);
+                    cross = __ballot_sync(ALL, part > 0 && below + above > target);
+                    const unsigned some = __ballot_sync(ALL, part > 0);
+                    const int who = cross ? __ffs(cross) - 1 : some ? 31 - __clz(some) : -1;
+                    if (lane == who) {
+                        const int per = (count + 31) >> 5, lo = lane * per, hi = min(count, lo + per);
+                        double run = below + (lane ? up : 0.0);
+                        bool crossed = false;
+                        for (int k = lo; k < hi; ++k) {
+                            const double v = at.draw(list[k], ep[k], at.y ? eq[k] : 0.0, residual);
+                            run += v;
+                            if (v > 0 && !crossed) next = list[k], crossed = run > target;
+                        }
+                    }
+                    if (who >= 0) next = __shfl_sync(ALL, next, who);
+                    below += __shfl_sync(ALL, above, 31);
+                } while (!whole && !cross && w < legal.words);
                 return true;
             };
             if (ALONE || !at.has_residual() || !draw(true)) draw(false);

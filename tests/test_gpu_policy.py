@@ -573,12 +573,14 @@ def check_verify(x, drafts, au, su, y=None, mask=None, lengths=None):
     w = torch.from_numpy(lps).cuda()
     tol = w.abs().nan_to_num() * U * 1.001 + 2.0 ** -40
     if mask is None:
-        # a kept draft's log Z comes from a 32-bit sum: per lane of at least eight warps n / 256 terms, each added once (u)
-        # and with an exponential of 4 u (2^-22) after three roundings of its argument (its size, weighted by the
-        # probabilities, is at most log2 n = 18: 3 * 18 u), 4 u for each of at most n / 1024 + 2 times that the maximum
-        # rises, and five joins of 5 u, in all below (2 n / 256 + 150) u
+        # a kept draft's log Z comes from a 32-bit sum.  These calls have at most 64 games, so a cluster has eight CTAs or
+        # at most 1,024 places for each, and a lane at most max(n / 256, 32) terms: each added once (u) and with an
+        # exponential of 4 u (2^-22) after three roundings of its argument (its size, weighted by the probabilities, is at
+        # most log2 n = 18: 3 * 18 u), 4 u for each of at most n / 1024 + 2 times that the maximum rises, and five joins of
+        # 5 u, in all below (2 max(n / 256, 32) + 150) u
+        assert x.shape[0] <= 64
         kept = torch.arange(out.shape[1], device="cuda")[None, :] < torch.from_numpy(acc).cuda()[:, None]
-        tol = tol + kept * ((2 * x.shape[2] / 256 + 150) * U)
+        tol = tol + kept * ((2 * max(x.shape[2] / 256, 32) + 150) * U)
     within(v.log_probs, w, tol, "log_probs")
     return v
 
@@ -612,6 +614,39 @@ def test_verify_drafts(dtype, games, d, n, density):
     ln = torch.randint(0, d + 1, (games,), generator=gen(3), device="cuda")
     check_verify(x, a, au, su, y if d else None, None if mask is None else mask.to(torch.uint8) * 200, ln)
     check_verify(x, a, au, su, None, mask, ln.to(torch.int32))
+
+
+@pytest.mark.parametrize("scored", [True, False])
+@pytest.mark.parametrize("layout", ["spread", "first", "last", "steps"])
+@pytest.mark.parametrize("d", [0, 3])
+def test_verify_drafts_longer_than_the_list(d, layout, scored):
+    """More legal actions than a warp's list holds (320), so that it takes them in parts: one more, exactly two and three
+    lists, parts that end inside a word of the mask, all actions; the points of the draw at both ends and in between."""
+    n = 5003
+    counts = [0, 1, 319, 320, 321, 345, 352, 639, 640, 641, 960, 961, 1500, n - 1, n]
+    games = 3 * len(counts)
+    x, _, au, su, y, _ = drafted(games, d, n, torch.float32, 40 + d, noise=0.7)
+    g = gen(50)
+    mask = torch.zeros(games, d + 1, n, dtype=torch.bool, device="cuda")
+    for k in range(games):
+        c = counts[k % len(counts)]
+        at = {"spread": torch.randperm(n, generator=g, device="cuda")[:c], "first": torch.arange(c, device="cuda"),
+              "last": torch.arange(n - c, n, device="cuda"),
+              "steps": torch.arange(c, device="cuda") * max(1, n // max(1, c))}[layout]
+        mask[k, :, at] = True
+    a = torch.where(mask[:, :d], y + x[:, :d], -torch.inf).argmax(-1).to(torch.int32)
+    su[:len(counts)], su[len(counts):2 * len(counts)] = 0, 1 - 2 ** -24
+    check_verify(x, a, au, su, y if d and scored else None, mask)
+    # NaN, +inf, rows of -inf and -inf but for the last part, in legal places behind the first list
+    last = n - 1 - mask.flip(-1).float().argmax(-1)
+    for k, v in ((4, float("nan")), (5, float("inf")), (12, float("-inf"))):
+        x[k, 0, last[k, 0]] = v
+    x[13] = -torch.inf
+    x[14, :, :n - 40] = -torch.inf
+    if d:
+        y[28, :, :n - 40] = -torch.inf
+        y[27, 0, last[27, 0]] = float("nan")
+    check_verify(x, a, au, su, y if d and scored else None, mask)
 
 
 def test_verify_drafts_of_the_target_itself_keeps_everything():
