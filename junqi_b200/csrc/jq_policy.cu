@@ -1011,17 +1011,19 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
         if (at.p.state == Dist::SOME && !at.broken()) {
             const float rf = d.sample_u[game];
             const double r = rf > 0.f ? (double)rf : 0.0;
-            if (at.has_residual() && !exact) make_exact();
+            if (at.has_residual() && at.y && !exact) make_exact();
             for (int pass = at.has_residual() ? 0 : 1; pass < 2; ++pass) {
                 const bool residual = pass == 0;
                 auto weight = [&](int j) { return at.draw(j, residual, table); };
                 double part = 0;
-                if (residual) {
+                if (residual && at.y) {
 #pragma unroll 4
                     for (int j = c0 + lane; j < c1; j += 32) part += weight(j);
                     part = warp_sum(part);
-                } else {
-                    part = chunk_sum64(at.x + c0, c1 - c0, lane, at.p, table);
+                } else {  // the target alone, but for the draft's action where that was certain
+                    const int skip = residual && at.act >= c0 && at.act < c1 ? at.act : c1;
+                    for (int from = c0, to = skip; from < c1; from = to + 1, to = c1)
+                        part += chunk_sum64(at.x + from, to - from, lane, at.p, table);
                 }
                 tell(part, 0);
                 // the first chunk whose running sum is above the point; with none, the last that has weight
@@ -1030,6 +1032,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 4) verify_dense_kernel(const Ve
                 turn ^= 1;
                 const double above = warp_scan(t0 + t1, lane), total = __shfl_sync(ALL, above, 31);
                 if (!exact && !residual) at.p.z = total;  // exp(x - m), summed up in 64 bits
+                if (residual && !at.y && !exact) at.p.z = total + at.p.weight(to_f(at.x[at.act]), table);
                 if (residual && !(total > RESIDUAL_MIN * at.scale(true))) continue;
                 const double target = r * total, up = __shfl_up_sync(ALL, above, 1), before = lane ? up : 0.0;
                 unsigned cross = __ballot_sync(ALL, t0 + t1 > 0 && above > target), some = __ballot_sync(ALL, t0 + t1 > 0);
