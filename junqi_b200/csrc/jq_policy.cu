@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // 64 bits (verify_dense_kernel).  Measured: 4,096 samples of 16,641 float32 with
 // up to 80 legal actions 20 us (69 MB, 3.4 TB/s), 8 games of 4 drafts 8.9 us,
 // 1,024 of up to 8 drafts 43 us; place by place and a CTA per game these took
-// 89, 33 and 125.  301 games of 5 drafts without a mask 77 us.
+// 89, 33 and 125.  301 games of 5 drafts without a mask 67 us.
 
 constexpr int VERIFY_WARPS = 36;  // of an SM, for the launch
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
