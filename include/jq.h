@@ -422,8 +422,9 @@ int jq_action_log_prob_backward(const void *d_logits, int64_t row_stride, int32_
  * 2^-40); after the last, from p at the place behind it.  Drawing takes the
  * least action whose running sum exceeds sample_u times the total.  What
  * comes out is distributed as the target's own play.  The actions are those
- * of 64-bit arithmetic; log-probabilities are rounded from it once, but those
- * of kept drafts without a mask come from 32-bit sums.
+ * of 64-bit arithmetic, with exponentials that are good to 2^-42 and 0 below
+ * e^-700; log-probabilities are rounded from it once, but those of kept drafts
+ * without a mask come from 32-bit sums.
  *
  * Outputs per game: `accepted` kept drafts; out_actions (drafts + 1): the
  * kept drafts, the drawn action, then -1; log_probs (drafts + 1): the

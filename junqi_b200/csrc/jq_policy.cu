@@ -548,7 +548,8 @@ struct Dist {
     __device__ __forceinline__ void start(float top, bool there) {
         state = !there || top == -INFINITY ? NONE : top < INFINITY ? SOME : BROKEN;
         m = state == SOME ? top : 0.f;
-        low = state == SOME ? (float)(m - 700.0) : INFINITY;  // (rounded to m itself where m is beyond 2^33: the next logit is far)
+        // rounded up: on the logits' own grid the nearest number may be as far as m - 1024, below what exp_near takes
+        low = state == SOME ? __double2float_ru(m - 700.0) : INFINITY;
         z = 0;
     }
     __device__ __forceinline__ double weight(float x, const double *table) const {  // exp(x - m)

@@ -83,8 +83,9 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, accept_u: torch.Te
     A drafted action is kept while accept_u q(a) < p(a); at the first that is
     not, the action is drawn from max(p - q, 0), after the last from p.  The
     actions that come out are distributed as if the target had played alone.
-    The choices are those of 64-bit arithmetic; log-probabilities are rounded from
-    it once (those of kept drafts without a mask come from 32-bit sums).  A place without legal
+    The choices are those of 64-bit arithmetic, with exponentials that are good to
+    2^-42 and 0 below e^-700; log-probabilities are rounded from it once (those of
+    kept drafts without a mask come from 32-bit sums).  A place without legal
     actions gives -1, one with NaN or +inf at a legal place -1 and a NaN
     log-probability.  Not differentiable: see :func:`action_log_prob`."""
     return Verified(*N.policy().verify_drafts(logits, drafts, accept_u, sample_u, draft_logits, mask, lengths))

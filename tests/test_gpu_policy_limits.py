@@ -1,0 +1,72 @@
+"""The policy operators at the ends of what they take."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from junqi_b200 import policy as P
+from tests.test_gpu_policy import DTYPES, U, check_verify, gen, within
+
+pytestmark = pytest.mark.gpu
+
+
+# -- logits of any size --------------------------------------------------------------
+
+@pytest.mark.parametrize("n,density", [(40, 0.6), (40, None), (2000, 0.7), (3000, None), (16641, 0.01), (16641, None)])
+@pytest.mark.parametrize("top", [2.2e9, 3e9, 8.6e9, 1e10, 6e8, 1.2e9, 2.0 ** 31, 2.0 ** 33, 5e12])
+def test_choices_among_logits_far_from_zero(top, n, density):
+    """Distances from the largest logit on both sides of 700, beyond which a weight is 0, of positive and of negative logits
+    (multiples of 64 or more, so none lies between 700 and 745, where the 64-bit exponential is not yet 0; a place that is
+    not one of the largest has a probability below 2^-360)."""
+    g = gen(int(top) % 1009 + n)
+    games, d = 12, 3
+    apart = torch.tensor([0, 256, 512, 640, 768, 832, 1024, 1280, 2048, 4096], device="cuda")
+    at = torch.randint(0, 10, (2, games, d + 1, n), generator=g, device="cuda")
+    sign = torch.where(torch.arange(games, device="cuda") % 2 == 0, 1.0, -1.0).double()[:, None, None]
+    x, y = ((sign * top - apart[k].double()).float() for k in at)
+    y = y[:, :d].contiguous()
+    mask = None if density is None else torch.rand(games, d + 1, n, generator=g, device="cuda") < density
+    best = x[:, :d] if mask is None else x[:, :d].masked_fill(~mask[:, :d], -torch.inf)
+    a = best.argmax(-1)
+    a[::3] = torch.randint(0, n, (len(a[::3]), d), generator=g, device="cuda")
+    au = 0.01 + 0.9 * torch.rand(games, d, generator=g, device="cuda")
+    su = torch.rand(games, generator=g, device="cuda")
+    check_verify(x, a, au, su, y, mask)
+    check_verify(x, a, au, su, None, mask)
+    check_verify(x[:, :1], a[:, :0], au[:, :0], su, None, None if mask is None else mask[:, :1])
+    s, lp = P.sample_actions(x, mask, torch.rand(games, d + 1, generator=g, device="cuda"))
+    legal = torch.ones_like(x, dtype=torch.bool) if mask is None else mask
+    some = legal.any(-1)
+    peak = x.masked_fill(~legal, -torch.inf).amax(-1)
+    assert torch.equal(s >= 0, some)
+    assert torch.equal(x.gather(2, s.clamp(min=0).long()[..., None])[..., 0][some], peak[some]), "not one of the largest"
+    ties = ((x == peak[..., None]) & legal).sum(-1)
+    within(lp[some], -ties[some].double().log(), 20 * U, "log_probs")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,masked", [(100, True), (100, False), (1500, True), (1500, False)])
+def test_choices_among_extreme_logits(dtype, n, masked):
+    """Legal places at -inf, at the type's lowest and highest values, all equal, and far apart."""
+    big = torch.finfo(dtype).max
+    x, y = (torch.randn(9, 3, n, generator=gen(s), device="cuda") for s in (4, 5))
+    x[0, :, :n // 2] = -torch.inf
+    x[1] = -torch.inf
+    x[2] = -big
+    x[3] = -big
+    x[3, :, 7] = 1.0
+    x[4] = 5.0
+    x[5, :, 10] = big
+    x[6, :, 20:] = -big
+    x[7] *= 1000
+    x[8], y[8] = big, -big
+    y[0], y[5] = -big, y[5].clone().index_fill_(1, torch.tensor([3], device="cuda"), big)
+    x, y = x.to(dtype), y[:, :2].to(dtype)
+    a = x[:, :2].argmax(-1)
+    a[::2, 1] = 10
+    au = torch.rand(9, 2, generator=gen(6), device="cuda").clamp(min=0.01)
+    su = torch.rand(9, generator=gen(7), device="cuda")
+    mask = torch.rand(9, 3, n, generator=gen(8), device="cuda") < 0.8 if masked else None
+    check_verify(x, a, au, su, y, mask)
+    check_verify(x, a, au, su, None, mask)
+    check_verify(x[:, :1], a[:, :0], au[:, :0], su, None, None if mask is None else mask[:, :1])
