@@ -84,6 +84,11 @@ void same_device(const char *what, const Tensor &x, std::initializer_list<const 
 Tensor last(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 // (rows, n) view (a copy only where the leading axes have no common stride).
 Tensor rows_of(const Tensor &t) { return last(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
+// The same inside a node's forward pass, where views have no history: with it, so that `once` finds the way back to `t`.
+Tensor saved_rows_of(const Tensor &t) {
+    at::AutoGradMode history(true);
+    return rows_of(t);
+}
 
 // `t` as contiguous int32 of `shape`; 64-bit values are cut to [lo, hi] first, so that none wraps.
 Tensor ints(const char *what, const Tensor &t, at::IntArrayRef shape, int64_t lo, int64_t hi) {
@@ -155,7 +160,7 @@ Tensor norm_forward(const Tensor &x, const Tensor &x2, const Tensor &weight, con
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const MaybeTensor &w, const MaybeTensor &b, double eps) {
         const Tensor weight = w.value_or(Tensor()), bias = b.value_or(Tensor());
-        const Tensor x2 = rows_of(x), stats = at::empty({x2.size(0), 3}, x.options().dtype(at::kFloat));
+        const Tensor x2 = saved_rows_of(x), stats = at::empty({x2.size(0), 3}, x.options().dtype(at::kFloat));
         ctx->save_for_backward({x2, weight, bias, stats});
         return norm_forward(x, x2, weight, bias, eps, stats);
     }
@@ -230,7 +235,7 @@ std::pair<Tensor, Tensor> logp_forward(const Tensor &logits, const Tensor &x2, c
 
 struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const MaybeTensor &mask, const Tensor &act) {
-        const Tensor x2 = rows_of(logits), m2 = mask ? rows_of(*mask) : Tensor();
+        const Tensor x2 = saved_rows_of(logits), m2 = mask ? rows_of(*mask) : Tensor();
         const int64_t rows = x2.size(0), n = x2.size(1);
         const Tensor stats = at::empty({rows, 4}, logits.options().dtype(at::kFloat));
         const Tensor bits = mask ? at::empty({rows, (n + 31) / 32}, logits.options().dtype(at::kInt)) : Tensor();

@@ -1,4 +1,5 @@
-"""The policy operators at the ends of what they take."""
+"""The policy operators at the ends of what they take: logits far from zero and far apart, derivatives of more than one
+order."""
 from __future__ import annotations
 
 import pytest
@@ -70,3 +71,54 @@ def test_choices_among_extreme_logits(dtype, n, masked):
     check_verify(x, a, au, su, y, mask)
     check_verify(x, a, au, su, None, mask)
     check_verify(x[:, :1], a[:, :0], au[:, :0], su, None, None if mask is None else mask[:, :1])
+
+
+# -- derivatives ---------------------------------------------------------------------------
+
+SHAPES = {"rows": lambda t: t, "boards": lambda t: t.view(2, 3, 8), "one": lambda t: t[0], "columns": lambda t: t.view(8, 6).t(),
+          "slice": lambda t: t[:, 1:7], "repeated": lambda t: t[:1].expand(4, 8), "four axes": lambda t: t.view(1, 3, 2, 8)}
+
+
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("op", ["norm", "logp", "entropy"])
+def test_second_derivatives_are_refused_whatever_the_shape(op, shape):
+    """A gradient that enters a penalty: its own derivative is an error, never left out of the sum."""
+    base = torch.randn(6, 8, generator=gen(1), device="cuda")
+    x = SHAPES[shape](base).detach()
+    if shape != "repeated":
+        x.requires_grad_(True)
+        leaf = x
+    else:
+        leaf = base[:1].clone().requires_grad_(True)
+        x = leaf.expand(4, 8)
+    if op == "norm":
+        loss = P.layer_norm(x, torch.ones(x.shape[-1], device="cuda")).square().sum()
+    else:
+        m = torch.rand(x.shape[-1], generator=gen(2), device="cuda") < 0.8
+        out = P.action_log_prob(x, m, torch.zeros(x.shape[:-1], dtype=torch.int32, device="cuda"))
+        loss = out[0 if op == "logp" else 1].sum()
+    (g,) = torch.autograd.grad(loss, leaf, create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(loss + g.square().sum(), leaf)
+
+
+@pytest.mark.parametrize("which", ["weight", "bias", "dy", "x of a linear layer"])
+def test_second_derivatives_of_the_other_inputs_are_refused(which):
+    x = torch.randn(2, 3, 8, generator=gen(1), device="cuda")
+    w, b = (torch.rand(8, generator=gen(s), device="cuda") for s in (2, 3))
+    dy = torch.randn(2, 3, 8, generator=gen(4), device="cuda")
+    lin = torch.rand(8, 8, generator=gen(5), device="cuda", requires_grad=True)
+    leaf = {"weight": w, "bias": b, "dy": dy, "x of a linear layer": lin}[which].requires_grad_(True)
+    h = x @ lin
+    y = P.layer_norm(h, w, b)
+    wrt = [v for v in (h, w, b) if v.requires_grad]
+    if which == "dy":
+        x.requires_grad_(True)
+        wrt, y = [x], P.layer_norm(x, w, b)
+    if which == "bias":  # no gradient depends on it, so there is nothing to refuse
+        (g,) = torch.autograd.grad(y, b, dy, create_graph=True)
+        return within(g, dy.double().sum((0, 1)), 8 * U * dy.abs().sum((0, 1)).double(), "db")
+    grads = torch.autograd.grad(y, wrt, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(sum(g.square().sum() for g in grads), leaf)
