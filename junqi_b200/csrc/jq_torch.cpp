@@ -80,6 +80,13 @@ void same_device(const char *what, const Tensor &x, std::initializer_list<const 
     REQUIRE(x.is_cuda(), what, ": needs CUDA tensors, got ", x.device());
 }
 
+// Forward-mode derivatives are not given: a tangent would be lost without a word.
+void no_tangent(const char *what, std::initializer_list<const Tensor *> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : inputs)
+        REQUIRE(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 // `t` with neighbouring places next to each other on its last axis.
 Tensor last(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 // (rows, n) view (a copy only where the leading axes have no common stride).
@@ -208,6 +215,7 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
                 " must be float32 or ", x.scalar_type(), ", got ", t.scalar_type());
     }
     REQUIRE(!weight || !bias || weight->scalar_type() == bias->scalar_type(), "layer_norm: weight and bias must have one type");
+    no_tangent("layer_norm", {&x, weight ? &*weight : &x, bias ? &*bias : &x});
     const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
     same_device("layer_norm", x, {&w, &b});
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
@@ -272,6 +280,7 @@ std::pair<Tensor, Tensor> action_log_prob(const Tensor &logits, const MaybeTenso
     const int64_t n = actions_of("action_log_prob", logits, 0);
     const Tensor act = ints("action_log_prob: actions", actions, logits.sizes().slice(0, logits.dim() - 1), -1, n);
     const Tensor m = mask_for("action_log_prob", mask, logits.sizes());
+    no_tangent("action_log_prob", {&logits});
     same_device("action_log_prob", logits, {&m, &act});
     if (at::GradMode::is_enabled() && logits.requires_grad()) {
         auto out = ActionLogProb::apply(logits, m.defined() ? MaybeTensor(m) : MaybeTensor(), act);

@@ -24,7 +24,7 @@ captured needs leaves that no earlier eager graph still refers to: release
 eager losses and outputs before the capture, as for any torch module.
 
 Nothing here falls back to torch: wrong arguments raise ValueError, a failed
-call RuntimeError.
+call RuntimeError.  Inputs with a forward-mode tangent are refused.
 """
 from __future__ import annotations
 
