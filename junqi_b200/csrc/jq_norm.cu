@@ -50,6 +50,7 @@ struct NormArgs {
 
 constexpr int NORM_E = 16, NORM_WARPS = 16;           // places of a thread, warps of the longest row
 constexpr int NORM_FWD_SLOTS = 4, NORM_BWD_SLOTS = 3; // of a warp's ring; a CTA's rows have 3
+constexpr int NORM_BWD_SLOT = 4688;                   // bytes, at most, where a slot has several rows: 2 x 8 x 3 of them on an SM
 
 // Sums of N values over the threads of a row.  TPR = 0: the row is the whole
 // CTA; two buffers, so one barrier per sum.
@@ -578,10 +579,13 @@ static NormPlan norm_plan(int64_t rows, int32_t dim, int es, int vec, int sms, b
         p.threads = 256, p.tpr = 2;
         while (p.tpr * NORM_E < dim) p.tpr *= 2;
         const int per = 32 / p.tpr;
-        // slots of 2 KB: copies in flight cover the latency, and a slot's cost is shared by several rows;
-        // but no more rows than there are for a warp
-        int64_t sets = 2048 / (per * (dense ? dim * es : row)), most = rows / (warps * per);
-        sets = sets < most ? sets : most;
+        // slots of 2 KB of x: copies in flight cover the latency, and a slot's cost is shared by several rows;
+        // but no more rows than there are for a warp, and in the backward pass, where a row has dy's and 12 bytes of
+        // statistics too, no more than let two CTAs' rings stand on an SM (short rows are mostly statistics)
+        const int bytes = dense ? dim * es : row;
+        int64_t sets = 2048 / (per * bytes), most = rows / (warps * per);
+        if (backward) most = min(most, (int64_t)(NORM_BWD_SLOT - 80) / (per * (2 * bytes + 12)));  // 80: three roundings up
+        sets = min(sets, most);
         p.chunk = per * (int)(sets < 1 ? 1 : sets);
         const int64_t need = (rows + 8 * (int64_t)p.chunk - 1) / (8 * (int64_t)p.chunk);
         p.grid = need < warps / 8 ? need : warps / 8;

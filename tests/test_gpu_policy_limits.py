@@ -1,12 +1,12 @@
 """The policy operators at the ends of what they take: logits far from zero and far apart, derivatives of more than one
-order."""
+order, rows of one or two places by the million."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from junqi_b200 import policy as P
-from tests.test_gpu_policy import DTYPES, U, check_verify, gen, within
+from tests.test_gpu_policy import DTYPES, U, check_norm, check_verify, gen, within
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,17 @@ def test_second_derivatives_of_the_other_inputs_are_refused(which):
     grads = torch.autograd.grad(y, wrt, dy, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(sum(g.square().sum() for g in grads), leaf)
+
+
+# -- layer norm's layouts -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [1, 2, 4, 7, 16])
+def test_layer_norm_short_rows_by_the_million(dtype, dim):
+    rows = 3_000_017
+    g = gen(dim)
+    x, dy = (torch.randn(rows, dim, generator=g, device="cuda").to(dtype) for _ in range(2))
+    w, b = (torch.rand(dim, generator=g, device="cuda") for _ in range(2))
+    check_norm(x, w, b, dy)
+    wide = torch.randn(rows, dim + 3, generator=g, device="cuda").to(dtype)
+    check_norm(wide[:, 1:1 + dim], w, None, dy)
