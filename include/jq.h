@@ -361,8 +361,9 @@ int jq_sample_softmax(const jq_batch *b, const int32_t *d_counts, const int32_t 
  * no counterpart in the reference, whose networks are torch modules.  Arrays
  * are device pointers, rows are `*_stride` elements apart with neighbouring
  * places next to each other (a stride of 0 repeats one row); outputs are
- * contiguous.  Aligned to their elements is enough; rows that all start on
- * 16 bytes take the widest loads.  Equal calls give equal bits.
+ * contiguous and overlap no input.  Aligned to their elements is enough;
+ * rows that all start on 16 bytes take the widest loads.  Equal calls give
+ * equal bits.
  * ------------------------------------------------------------------------- */
 
 /* Element types of features, logits and weights. */

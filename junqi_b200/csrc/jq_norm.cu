@@ -22,8 +22,11 @@
 // Statistics are 32-bit.  The mean is taken twice: m, the rounded mean, then
 // delta = mean(x - m), what the rounding left, so a row whose mean is large
 // against its spread loses nothing (s2 = mean((x - m)^2) - delta^2, in which
-// delta^2 is at rounding level).  The three numbers (m, delta, r) per row go
-// to the backward pass.
+// delta^2 is at rounding level).  Where it is not, because the row is all but
+// constant, m takes delta in and the row is done once more, from memory, when a
+// warp (CTA) has been through all of its rows: asked for in the walk itself, it
+// cost every row 1 to 20 % by the registers.  The three numbers (m, delta, r)
+// per row go to the backward pass.
 //
 // Measured (B200, 264,192 rows of 256 bfloat16): forward 47 us (5.8 TB/s, 0.89
 // of a plain copy's rate), backward 70 us (5.8 TB/s) and 3 us for the second
@@ -76,6 +79,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*sm)[NORM_WARPS][N
     }
 }
 
+// Whether the rounding of the mean is most of what the squares about it show,
+// or made them overflow: a row that is all but constant.
+__device__ __forceinline__ bool is_off(float var, float square) { return var < 0.75f * square || square == INFINITY; }
+
 // A row's places in one thread, as pairs of floats: E / VEC packs, the row's
 // threads apart, in groups of G places.  A row takes as few threads as hold
 // it, so its first half is inside the row for every thread, and at most the
@@ -89,6 +96,8 @@ struct Places {
         return FULL || (TPR == 2 ? g < groups : G == NORM_E / 2 || g < NG - 1 || groups == NG);
     }
     static constexpr bool sure(int pack) { return FULL || (TPR != 2 && pack < NORM_E / VEC / 2); }
+    // places outside the row: 0, or as its last ones
+    template <bool LAST = false>
     __device__ __forceinline__ void load(const char *row, int t, int tpr, int dim, int groups) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -96,7 +105,8 @@ struct Places {
                 alignas(16) T e[G];
 #pragma unroll
                 for (int k = 0; k < PG; ++k) {
-                    const int j = (t + (g * PG + k) * tpr) * VEC;
+                    int j = (t + (g * PG + k) * tpr) * VEC;
+                    if (LAST) j = min(j, dim - VEC);
                     Pack<T, VEC> p;
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) p.v[i] = from_f<T>(0.f);
@@ -188,9 +198,35 @@ struct NormFwd {
     float (*sm2)[NORM_WARPS][2];
     int phase1 = 0, phase2 = 0;
 
-    __device__ __forceinline__ void row(const char *from, uint32_t r, bool valid) {
+    // x - m; the mean of that, and of its square
+    __device__ __forceinline__ void centre(P &x, float m, float &delta, float &square) {
+        const float inv = 1.f / (float)a.dim;
+        const bool whole = FULL || NORM_E * tpr == a.dim;
+        const f2 nm = both(-m);
+        f2 u = both(0.f), v = both(0.f);
+#pragma unroll
+        for (int g = 0; g < P::NG; ++g)
+            if (P::has(g, a.groups))
+#pragma unroll
+                for (int i = g * P::G / 2; i < (g + 1) * P::G / 2; ++i) {
+                    x.v[i] = x.v[i] + nm;
+                    if (!whole && !P::sure(2 * i / VEC)) {
+                        float2 c = parts(x.v[i]);
+                        if ((t + 2 * i / VEC * tpr) * VEC >= a.dim) c.x = 0.f;
+                        if ((t + (2 * i + 1) / VEC * tpr) * VEC >= a.dim) c.y = 0.f;
+                        x.v[i] = make_f2(c.x, c.y);
+                    }
+                    u = u + x.v[i];
+                    v = fma2(x.v[i], x.v[i], v);
+                }
+        float s2[2] = {parts(u).x + parts(u).y, parts(v).x + parts(v).y};
+        row_sum<TPR>(s2, sm2, phase2);
+        delta = s2[0] * inv, square = s2[1] * inv;
+    }
+    // AGAIN: only rows that are off, with a better mean.  Whether the row is (behind the last row: whatever).
+    template <bool AGAIN>
+    __device__ __forceinline__ bool row(const char *from, uint32_t r, bool valid) {
         const int dim = a.dim, groups = a.groups;
-        const float inv = 1.f / (float)dim;
         P x;
         x.load(from, t, tpr, dim, groups);
         f2 s = both(0.f);
@@ -201,39 +237,25 @@ struct NormFwd {
                 for (int i = g * P::G / 2; i < (g + 1) * P::G / 2; ++i) s = s + x.v[i];
         float s1[1] = {parts(s).x + parts(s).y};
         row_sum<TPR>(s1, sm1, phase1);
-        const float m = s1[0] * inv;
-        const f2 nm = both(-m);
-        const bool whole = FULL || NORM_E * tpr == dim;
-        f2 u = both(0.f), v = both(0.f);
-#pragma unroll
-        for (int g = 0; g < P::NG; ++g)
-            if (P::has(g, groups))
-#pragma unroll
-                for (int i = g * P::G / 2; i < (g + 1) * P::G / 2; ++i) {
-                    x.v[i] = x.v[i] + nm;
-                    if (!whole && !P::sure(2 * i / VEC)) {
-                        float2 c = parts(x.v[i]);
-                        if ((t + 2 * i / VEC * tpr) * VEC >= dim) c.x = 0.f;
-                        if ((t + (2 * i + 1) / VEC * tpr) * VEC >= dim) c.y = 0.f;
-                        x.v[i] = make_f2(c.x, c.y);
-                    }
-                    u = u + x.v[i];
-                    v = fma2(x.v[i], x.v[i], v);
-                }
-        float s2[2] = {parts(u).x + parts(u).y, parts(v).x + parts(v).y};
-        row_sum<TPR>(s2, sm2, phase2);
-        const float delta = s2[0] * inv;
-        const float q = rsqrtf(fmaxf(s2[1] * inv - delta * delta, 0.f) + a.eps);  // 2 units: no more than the sums
+        float m = s1[0] * (1.f / (float)dim), delta, square;
+        centre(x, m, delta, square);
+        if (AGAIN) {
+            valid = valid && is_off(fmaxf(square - delta * delta, 0.f), square);
+            m += delta;
+            x.load(from, t, tpr, dim, groups);
+            centre(x, m, delta, square);
+        }
+        const float var = fmaxf(square - delta * delta, 0.f), q = rsqrtf(var + a.eps);  // 2 units: no more than the sums
         if (valid) {
             T *y = (T *)((char *)a.y + (uint64_t)r * (uint32_t)(dim * (int)sizeof(T)));
-            const f2 rr = both(q), off = both(-delta * q);
+            const f2 rr = both(q), back = both(-delta * q);
 #pragma unroll
             for (int g = 0; g < P::NG; ++g)
                 if (P::has(g, groups)) {
                     f2 o[P::G / 2];
 #pragma unroll
                     for (int i = 0; i < P::G / 2; ++i)
-                        o[i] = fma2(fma2(x.v[g * P::G / 2 + i], rr, off), w[g * P::G / 2 + i], b[g * P::G / 2 + i]);
+                        o[i] = fma2(fma2(x.v[g * P::G / 2 + i], rr, back), w[g * P::G / 2 + i], b[g * P::G / 2 + i]);
                     store_group<T, VEC, TPR, FULL>(y, o, g, t, tpr, dim);
                 }
             if (a.stats && t == 0) {
@@ -241,6 +263,7 @@ struct NormFwd {
                 st[0] = m, st[1] = delta, st[2] = q;
             }
         }
+        return is_off(var, square);
     }
 };
 
@@ -269,6 +292,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) fetch(s);
     int slot = 0;
+    bool again = false;
     for (uint32_t r0 = first; r0 < rows; r0 += step) {
         const int free = slot == 0 ? S - 1 : slot - 1;
         const char *at = ring + slot * a.slot_bytes;
@@ -278,18 +302,24 @@ __global__ void __launch_bounds__(TPR ? 256 : 768, TPR ? 3 : 1) norm_fwd_kernel(
             __syncwarp();
             for (uint32_t q = 0; q < chunk; q += PER) {  // whole warps: every lane takes part in the shuffles
                 const uint32_t mine = q + lane / (TPR ? TPR : 32);
-                k.row(xs.row(at, r0, mine), r0 + mine, r0 + mine < rows);  // behind the last row: whatever is there, for nobody
+                again |= k.template row<false>(xs.row(at, r0, mine), r0 + mine, r0 + mine < rows);  // behind the last row: whatever is there, for nobody
             }
             __syncwarp();
         } else {
             copies_wait_but<S - 2>();
             __syncthreads();  // this row has arrived, and the last one's slot has been read
             fetch(free);
-            k.row(xs.row(at, r0, 0), r0, true);
+            again |= k.template row<false>(xs.row(at, r0, 0), r0, true);
         }
         slot = slot + 1 == S ? 0 : slot + 1;
     }
     copies_wait_but<0>();
+    if (!(TPR ? __any_sync(ALL, again) : again)) return;
+    for (uint32_t r0 = first; r0 < rows; r0 += step)
+        for (uint32_t q = 0; q < chunk; q += PER) {
+            const uint32_t r = r0 + q + (TPR ? lane / (TPR ? TPR : 32) : 0);
+            k.template row<true>((const char *)a.x + min(r, rows - 1) * a.x_stride * (int64_t)sizeof(T), r, r < rows);
+        }
 }
 
 template <typename T, int VEC, int TPR, bool FULL>
@@ -301,16 +331,19 @@ struct NormBwd {
     float (*sm)[NORM_WARPS][2];
     int phase = 0;
 
-    __device__ __forceinline__ void row(const char *fx, const char *fy, const float *st, uint32_t r, bool valid) {
+    // Places outside the row have dy = 0 and x = 0, so no part in any sum while their xh is a number.  It is not where the
+    // mean is that large against the spread; AGAIN: dx of such rows, with other places in theirs.  Whether the row may be one.
+    template <bool AGAIN>
+    __device__ __forceinline__ bool row(const char *fx, const char *fy, const float *st, uint32_t r, bool valid) {
         const int dim = a.dim, groups = a.groups;
         const float inv = 1.f / (float)dim;
         P x, d;
-        x.load(fx, t, tpr, dim, groups);
+        x.template load<AGAIN>(fx, t, tpr, dim, groups);
         d.load(fy, t, tpr, dim, groups);
         const float q = st[2];
+        if (AGAIN) valid = valid && !(fabsf(st[0] * q) < 1e38f);
         const f2 nm = both(-st[0]), rr = both(q), off = both(-st[1] * q);
         f2 s = both(0.f), v = both(0.f);
-        // places outside the row have dy = 0 and x = 0: a finite xh, and no part in any sum
 #pragma unroll
         for (int g = 0; g < P::NG; ++g)
             if (P::has(g, groups))
@@ -320,10 +353,11 @@ struct NormBwd {
                     const f2 gg = d.v[i] * w[i];
                     s = s + gg;
                     v = fma2(gg, x.v[i], v);
+                    if (AGAIN) continue;
                     aw[i] = fma2(d.v[i], x.v[i], aw[i]);
                     ab[i] = ab[i] + d.v[i];
                 }
-        if (!a.y) return;
+        if (!a.y) return false;
         float sums[2] = {parts(s).x + parts(s).y, parts(v).x + parts(v).y};
         row_sum<TPR>(sums, sm, phase);
         if (valid) {
@@ -341,8 +375,26 @@ struct NormBwd {
                     store_group<T, VEC, TPR, FULL>(dx, o, g, t, tpr, dim);
                 }
         }
+        return !FULL && sums[1] != sums[1];
     }
 };
+
+// dx of the warp's (CTA's) rows whose xh is no number outside the row.  Out of line, the walk keeps its registers.
+template <typename T, int VEC, int TPR>
+__device__ __noinline__ void norm_bwd_again(const NormArgs a, uint32_t first, uint32_t step, float (*sm)[NORM_WARPS][2]) {
+    constexpr int PER = 32 / (TPR ? TPR : 32);
+    const uint32_t lane = threadIdx.x & 31, rows = (uint32_t)a.rows, chunk = TPR ? a.chunk : 1;
+    if (!TPR) __syncthreads();  // the walk's sums have been read
+    NormBwd<T, VEC, TPR, false> k{a, TPR ? (int)lane & (TPR - 1) : (int)threadIdx.x, TPR ? TPR : (int)blockDim.x};
+    k.sm = sm;
+    load_weights<T, VEC>(k.w, a.w, a.wf32, 1.f, k.t, k.tpr, a.dim);
+    for (uint32_t r0 = first; r0 < rows; r0 += step)
+        for (uint32_t q = 0; q < chunk; q += PER) {
+            const uint32_t mine = r0 + q + (TPR ? lane / (TPR ? TPR : 32) : 0), r = min(mine, rows - 1);
+            k.template row<true>((const char *)a.x + r * a.x_stride * (int64_t)sizeof(T), (const char *)a.dy + r * a.dy_stride * (int64_t)sizeof(T),
+                                 a.stats + (uint64_t)r * 3, r, mine < rows);
+        }
+}
 
 // 16 warps an SM by registers.
 template <typename T, int VEC, int TPR, bool FULL>
@@ -380,8 +432,9 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
         copies_end_group();
         xs.skip(), ys.skip(), ahead += step;
     };
+    bool again = false;
     auto row = [&](const char *at, uint32_t r0, uint32_t q, bool valid) {
-        k.row(xs.row(at, r0, q), ys.row(at + a.x_bytes, r0, q), (const float *)(at + 2 * a.x_bytes) + 3 * q, r0 + q, valid);
+        again |= k.template row<false>(xs.row(at, r0, q), ys.row(at + a.x_bytes, r0, q), (const float *)(at + 2 * a.x_bytes) + 3 * q, r0 + q, valid);
     };
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) fetch(s);
@@ -404,8 +457,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
         slot = slot + 1 == S ? 0 : slot + 1;
     }
     copies_wait_but<0>();
-    if (!a.part) return;
-    if (TPR) {
+    if (a.part && TPR) {
         const int sub = lane / (TPR ? TPR : 32);
         // the CTA's rows: those of a warp by shuffles, then its eight warps, in the ring's memory
         __syncthreads();
@@ -429,7 +481,7 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
             for (int i = 0; i < 8; ++i) u += cw[i * dim + j], v += cb[i * dim + j];
             out[j] = u, out[dim + j] = v;
         }
-    } else {
+    } else if (a.part) {
 #pragma unroll
         for (int e = 0; e < NORM_E; ++e) {
             const int j = (k.t + e / VEC * k.tpr) * VEC + e % VEC;
@@ -437,6 +489,8 @@ __global__ void __launch_bounds__(TPR ? 256 : 512, TPR ? 2 : 1) norm_bwd_kernel(
             if (j < dim) out[j] = e % 2 ? u.y : u.x, out[dim + j] = e % 2 ? v.y : v.x;
         }
     }
+    if constexpr (!FULL)
+        if (TPR ? __any_sync(ALL, again) : again) norm_bwd_again<T, VEC, TPR>(a, first, step, sm);
 }
 
 // Sums of the weights' gradients over the CTAs, in a fixed order and 64 bits;
@@ -477,7 +531,7 @@ __global__ void __launch_bounds__(512) norm_dw_kernel(const float *part, int par
 // each sum (from L2, where one row stays), and for the weights' gradients a
 // thread per column over a share of the rows.
 template <typename T>
-__global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(512, 4) norm_fwd_long_kernel(const NormArgs a) {
     __shared__ float sm1[2][NORM_WARPS][1], sm2[2][NORM_WARPS][2];
     pdl_enter();
     const float inv = 1.f / (float)a.dim;
@@ -485,27 +539,32 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormArgs a) {
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = (const T *)a.x + row * a.x_stride;
         T *y = (T *)a.y + row * a.dim;
-        float s1[1] = {0.f}, s2[2] = {0.f, 0.f};
+        float s1[1] = {0.f}, s2[2];
 #pragma unroll 8
         for (int j = threadIdx.x; j < a.dim; j += 512) s1[0] += to_f(x[j]);
         row_sum<0>(s1, sm1, phase1);
-        const float m = s1[0] * inv;
+        float m = s1[0] * inv;
+        for (bool last = false;; last = true) {
+            s2[0] = s2[1] = 0.f;
 #pragma unroll 8
-        for (int j = threadIdx.x; j < a.dim; j += 512) {
-            const float c = to_f(x[j]) - m;
-            s2[0] += c;
-            s2[1] += c * c;
-        }
-        row_sum<0>(s2, sm2, phase2);
-        const float delta = s2[0] * inv;
-        const float r = 1.f / sqrtf(fmaxf(s2[1] * inv - delta * delta, 0.f) + a.eps);
+            for (int j = threadIdx.x; j < a.dim; j += 512) {
+                const float c = to_f(x[j]) - m;
+                s2[0] += c;
+                s2[1] += c * c;
+            }
+            row_sum<0>(s2, sm2, phase2);
+            const float delta = s2[0] * inv, square = s2[1] * inv;
+            const float var = fmaxf(square - delta * delta, 0.f), r = 1.f / sqrtf(var + a.eps);
 #pragma unroll 4
-        for (int j = threadIdx.x; j < a.dim; j += 512)
-            y[j] = from_f<T>(((to_f(x[j]) - m) - delta) * r * (a.w ? load_as<T>(a.w, a.wf32, j) : 1.f) +
-                             (a.b ? load_as<T>(a.b, a.wf32, j) : 0.f));
-        if (a.stats && threadIdx.x == 0) {
-            float *st = a.stats + row * 3;
-            st[0] = m, st[1] = delta, st[2] = r;
+            for (int j = threadIdx.x; j < a.dim; j += 512)
+                y[j] = from_f<T>(((to_f(x[j]) - m) - delta) * r * (a.w ? load_as<T>(a.w, a.wf32, j) : 1.f) +
+                                 (a.b ? load_as<T>(a.b, a.wf32, j) : 0.f));
+            if (a.stats && threadIdx.x == 0) {
+                float *st = a.stats + row * 3;
+                st[0] = m, st[1] = delta, st[2] = r;
+            }
+            if (__builtin_expect(last || !is_off(var, square), 1)) break;
+            m += delta;
         }
     }
 }

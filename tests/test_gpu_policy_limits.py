@@ -1,5 +1,5 @@
-"""The policy operators at the ends of what they take: logits far from zero and far apart, derivatives of more than one
-order, rows of one or two places by the million."""
+"""The policy operators at the ends of what they take: logits far from zero and far apart, derivatives of more than
+one order, rows of one or two places by the million, large constant rows."""
 from __future__ import annotations
 
 import pytest
@@ -136,3 +136,34 @@ def test_layer_norm_short_rows_by_the_million(dtype, dim):
     check_norm(x, w, b, dy)
     wide = torch.randn(rows, dim + 3, generator=g, device="cuda").to(dtype)
     check_norm(wide[:, 1:1 + dim], w, None, dy)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [60, 200, 708, 1111, 2047, 7356, 8191, 9001])
+def test_layer_norm_large_constant_rows(dtype, dim):
+    """A row of one number has no spread: its result is the bias whatever the number, and its gradients are those of a row
+    of zeros (a mean in 64 bits would not show it: rounded, it misses a number of 24 bits of that size by more than eps).
+    Beside them rows of two neighbouring numbers, and large numbers whose squares overflow."""
+    rows = 400
+    g = gen(dim)
+    x = (10 ** (3 + 15 * torch.rand(rows, 1, generator=g, device="cuda", dtype=torch.float64))).to(dtype)
+    x = x * torch.where(torch.arange(rows, device="cuda") % 2 == 0, 1, -1).to(dtype)[:, None]
+    x[0], x[1], x[2] = 3e33, -1e34, 1e38 / dim
+    x = x.expand(rows, dim).contiguous()
+    w, b = (torch.rand(dim, generator=g, device="cuda") for _ in range(2))
+    dy = torch.randn(rows, dim, generator=g, device="cuda").to(dtype)
+    z = x.requires_grad_(True)
+    o = torch.zeros_like(x).requires_grad_(True)
+    w.requires_grad_(True)
+    b.requires_grad_(True)
+    y = P.layer_norm(z, w, b)
+    assert torch.equal(y, b.to(dtype).expand(rows, dim))
+    of_zeros = torch.autograd.grad(P.layer_norm(o, w, b), (o, w, b), dy)
+    for got, want in zip(torch.autograd.grad(y, (z, w, b), dy), of_zeros):
+        assert torch.equal(got, want)
+    x = x.detach()
+    check_norm(torch.zeros_like(x), w, b, dy)
+    if dtype == torch.float32:
+        big = x[:, :1].clamp(-1e12, 1e12).clone()
+        two = torch.where(torch.rand(rows, dim, generator=g, device="cuda") < 0.5, big, torch.nextafter(big, 2 * big))
+        check_norm(two, w, b, dy)
