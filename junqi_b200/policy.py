@@ -85,7 +85,8 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, accept_u: torch.Te
     actions that come out are distributed as if the target had played alone.
     The choices are those of 64-bit arithmetic, with exponentials that are good to
     2^-42 and 0 below e^-700; log-probabilities are rounded from it once (those of
-    kept drafts without a mask come from 32-bit sums).  A place without legal
+    kept drafts without a mask come from 32-bit sums: off by (92 + 6 n / 256) 2^-24
+    at most, measured below 2^-17 up to 262,144 actions).  A place without legal
     actions gives -1, one with NaN or +inf at a legal place -1 and a NaN
     log-probability.  Not differentiable: see :func:`action_log_prob`."""
     return Verified(*N.policy().verify_drafts(logits, drafts, accept_u, sample_u, draft_logits, mask, lengths))

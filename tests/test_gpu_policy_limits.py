@@ -167,3 +167,27 @@ def test_layer_norm_large_constant_rows(dtype, dim):
         big = x[:, :1].clamp(-1e12, 1e12).clone()
         two = torch.where(torch.rand(rows, dim, generator=g, device="cuda") < 0.5, big, torch.nextafter(big, 2 * big))
         check_norm(two, w, b, dy)
+
+
+# -- kept drafts without a mask ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("games,n", [(1, 262144), (64, 40000), (700, 262144), (700, 16641), (640, 33)])
+def test_log_probabilities_of_kept_drafts_of_any_number_of_games(games, n, dtype):
+    """Their log Z is of 32 bits: an exponential is off by 4 u, its argument's three roundings by 3 * 18 u on average (log2 n
+    <= 18), nine additions before a sum joins its lane's; a lane has at most n / 256 of those (eight places or more each), whose
+    addition and factor for a risen maximum cost 6 u; five joins of 5 u.  With 700 games a row is one CTA's.  Rising rows
+    raise the maximum at every step."""
+    g = gen(games + n)
+    x = torch.randn(games, 2, n, generator=g, device="cuda").mul_(2)
+    x[0::4, 0] = torch.linspace(-6, 3, n, device="cuda")
+    x[1::4, 0] = torch.linspace(4, -5, n, device="cuda")
+    x[2::4, 0] = -0.3
+    x = x.to(dtype)
+    a = torch.randint(0, n, (games, 1), generator=g, device="cuda")
+    v = P.verify_drafts(x, a, torch.zeros(games, 1, device="cuda"), torch.rand(games, generator=g, device="cuda"))
+    assert (v.accepted == 1).all() and torch.equal(v.actions[:, :1].long(), a)
+    for k in range(0, games, 100):
+        xd = x[k:k + 100, 0].double()
+        want = xd.gather(1, a[k:k + 100])[:, 0] - xd.logsumexp(1)
+        within(v.log_probs[k:k + 100, 0], want, 1.01 * (92 + 6 * max(n / 256, 1) + want.abs()) * U, "log_probs")
