@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "jq_host.cuh"
 
@@ -64,11 +65,14 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
 }
 __device__ __forceinline__ f2 to_f2(const float *v) { return make_f2(v[0], v[1]); }
 __device__ __forceinline__ f2 to_f2(const __half *v) {
-    const float2 p = __half22float2(*(const __half2 *)v);
+    __half2 h;
+    memcpy(&h, v, 4);
+    const float2 p = __half22float2(h);
     return make_f2(p.x, p.y);
 }
 __device__ __forceinline__ f2 to_f2(const __nv_bfloat16 *v) {
-    const uint32_t u = *(const uint32_t *)v;  // a bfloat16 is the upper half of its float
+    uint32_t u;
+    memcpy(&u, v, 4);  // a bfloat16 is the upper half of its float
     return make_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 __device__ __forceinline__ void from_f2(float *v, f2 a) {
@@ -77,11 +81,13 @@ __device__ __forceinline__ void from_f2(float *v, f2 a) {
 }
 __device__ __forceinline__ void from_f2(__half *v, f2 a) {
     const float2 p = parts(a);
-    *(__half2 *)v = __floats2half2_rn(p.x, p.y);
+    const __half2 h = __floats2half2_rn(p.x, p.y);
+    memcpy(v, &h, 4);
 }
 __device__ __forceinline__ void from_f2(__nv_bfloat16 *v, f2 a) {
     const float2 p = parts(a);
-    *(__nv_bfloat162 *)v = __floats2bfloat162_rn(p.x, p.y);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);
+    memcpy(v, &h, 4);
 }
 
 // Asynchronous copies into shared memory, in groups that complete in order.

@@ -528,15 +528,15 @@ __device__ __forceinline__ double exp_table(int i) { return exp2((double)i / EXP
 // 16 / ln 2, -ln 2 / 16, 1 / 5!, 1 / 4!, 1 / 3!: as constants in memory they are operands; written into the code,
 // each use takes two more instructions to make one
 __constant__ double c_exp[5] = {EXP_STEPS * 1.4426950408889634, -0.69314718055994531 / EXP_STEPS, 1.0 / 120, 1.0 / 24, 1.0 / 6};
-__device__ __forceinline__ double exp_near(double d, const double *table) {  // d in [-700, 0]
+__device__ __forceinline__ double exp_near(double d, const double *table) {  // d in [-700, 0]; elsewhere some number
     static_assert(EXP_STEPS == 16, "four bits of k are the table's");
     constexpr double MAGIC = 1.5 * 4503599627370496.0;  // 1.5 * 2^52: a sum's last bit is 1
     const double near = fma(d, c_exp[0], MAGIC);
-    const int k = __double2loint(near);
+    const uint32_t k = (uint32_t)__double2loint(near);  // k in two's complement
     const double r = fma(near - MAGIC, c_exp[1], d);
     const double e = r * fma(r, fma(r, fma(r, fma(r, c_exp[2], c_exp[3]), c_exp[4]), 0.5), 1.0);
     const double at = table[k & 15], v = fma(at, e, at);
-    return __hiloint2double(__double2hiint(v) + ((k & ~15) << 16), __double2loint(v));
+    return __hiloint2double((int)((uint32_t)__double2hiint(v) + ((k & ~15u) << 16)), __double2loint(v));
 }
 
 // One row of logits and what its probabilities need.
@@ -545,6 +545,7 @@ struct Dist {
     double m, z;  // the largest logit, and Z
     float low;    // logits below it have exp(x - m) = 0
     int state;
+    static __device__ __forceinline__ Dist none() { return {0.0, 0.0, INFINITY, NONE}; }
     __device__ __forceinline__ void start(float top, bool there) {
         state = !there || top == -INFINITY ? NONE : top < INFINITY ? SOME : BROKEN;
         m = state == SOME ? top : 0.f;
@@ -569,7 +570,8 @@ struct Place {
     Dist p, q;
     __device__ __forceinline__ Place(const jq_drafts &d, int game, int i, int len)
         : x((const T *)d.logits + game * d.logits_game + i * d.logits_place), y(nullptr),
-          mask(d.mask ? d.mask + game * d.mask_game + i * d.mask_place : nullptr), act(-1), drafted(i < len), u(0.f), xa(0.f), ya(0.f) {
+          mask(d.mask ? d.mask + game * d.mask_game + i * d.mask_place : nullptr), act(-1), drafted(i < len), u(0.f), xa(0.f), ya(0.f),
+          p(Dist::none()), q(Dist::none()) {
         if (drafted) {
             act = d.drafted[(int64_t)game * d.drafts + i];
             u = d.accept_u[(int64_t)game * d.drafts + i];
