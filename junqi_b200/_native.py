@@ -7,8 +7,10 @@ status, a ``RuntimeError`` carrying ``jq_last_error()`` is raised.
 from __future__ import annotations
 
 import ctypes
+import importlib.metadata
 import importlib.util
 import subprocess
+import sys
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -130,9 +132,19 @@ def build(force: bool = False, trace: bool = False) -> Path:
         need[POLICY_PATH] = list(CSRC.glob("*.cpp")) + [header]
     stale = any(not out.exists() or any(p.stat().st_mtime > out.stat().st_mtime for p in srcs)
                 for out, srcs in need.items())
-    if force or stale:
-        subprocess.run(["make", "-s", "-C", str(CSRC)] + (["trace"] if trace else []), check=True)
+    other = not trace and POLICY_PATH.exists() and not _policy_is_ours()
+    if other:
+        POLICY_PATH.unlink()  # file times do not show it
+    if force or stale or other:
+        subprocess.run(["make", "-s", "-C", str(CSRC), f"PYTHON={sys.executable}"] + (["trace"] if trace else []),
+                       check=True)
     return path
+
+
+def _policy_is_ours() -> bool:
+    """Whether _policy.so was built for this interpreter's ABI and this torch: it carries both as a text."""
+    ours = f"junqi_b200 built for {sys.implementation.cache_tag} torch-{importlib.metadata.version('torch')}\0"
+    return ours.encode() in POLICY_PATH.read_bytes()
 
 
 _lib = None
@@ -172,6 +184,8 @@ def policy():
     if _policy is None:
         if not POLICY_PATH.exists():
             raise RuntimeError(f"{POLICY_PATH.name} not built at {POLICY_PATH}; run junqi_b200._native.build()")
+        if not _policy_is_ours():
+            raise RuntimeError(f"{POLICY_PATH} was built for another Python or torch; run junqi_b200._native.build()")
         L = lib()
         spec = importlib.util.spec_from_file_location("junqi_b200._policy", POLICY_PATH)
         mod = importlib.util.module_from_spec(spec)

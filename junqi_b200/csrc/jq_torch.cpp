@@ -349,6 +349,7 @@ std::pair<Tensor, Tensor> sample_actions(const Tensor &logits, const MaybeTensor
 }  // namespace
 
 PYBIND11_MODULE(_policy, m) {
+    m.attr("built_for") = "junqi_b200 built for " JQ_BUILT_FOR;
     const auto free = py::call_guard<py::gil_scoped_release>();
     m.def("bind", &bind);
     m.def("layer_norm", &layer_norm, free);

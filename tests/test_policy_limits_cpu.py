@@ -1,10 +1,14 @@
-"""Refusals of the policy operators that need no GPU, at the ends of what they take."""
+"""The policy operators' refusals that need no GPU, at the ends of what they take, and the build of their binding."""
 from __future__ import annotations
+
+import importlib.metadata
+import sys
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from junqi_b200 import _native as N
 from junqi_b200 import policy as P
 
 
@@ -32,3 +36,19 @@ def test_forward_mode_is_refused(which, needs_grad):
             call()
     with pytest.raises(ValueError, match="CUDA"):
         call()
+
+
+def test_the_binding_is_built_for_this_interpreter_and_torch(tmp_path, monkeypatch):
+    """`make` gets the running interpreter; a binding of another Python or torch is refused, and built anew."""
+    assert N._policy_is_ours()
+    assert N.policy().built_for.endswith(f"{sys.implementation.cache_tag} torch-{importlib.metadata.version('torch')}")
+    other = tmp_path / "_policy.so"
+    other.write_bytes(N.POLICY_PATH.read_bytes().replace(importlib.metadata.version("torch").encode() + b"\0", b"0.0\0"))
+    calls = []
+    monkeypatch.setattr(N, "POLICY_PATH", other)
+    monkeypatch.setattr(N, "_policy", None)
+    monkeypatch.setattr(N.subprocess, "run", lambda cmd, check: calls.append(cmd))
+    with pytest.raises(RuntimeError, match="another Python or torch"):
+        N.policy()
+    N.build()
+    assert not other.exists() and f"PYTHON={sys.executable}" in calls[0]
