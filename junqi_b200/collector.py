@@ -103,7 +103,7 @@ class RolloutCollector:
     def _answer(self):
         env = self.env
         sp, gl = env.observe(None, seats_per_env=1)
-        return self.policy(sp, gl, env.mask.view(torch.bool))
+        return tuple(self.policy(sp, gl, env.mask.view(torch.bool)))
 
     def _act(self):
         out = self._answer()

@@ -52,3 +52,21 @@ def test_the_binding_is_built_for_this_interpreter_and_torch(tmp_path, monkeypat
         N.policy()
     N.build()
     assert not other.exists() and f"PYTHON={sys.executable}" in calls[0]
+
+
+@pytest.mark.parametrize("kind", [tuple, list, iter, lambda out: (v for v in out), torch.stack])
+def test_the_collector_takes_what_can_be_unpacked(kind):
+    """(action, log_prob, value) in whatever form a policy returns it: an iterator has no length, and no last element."""
+    from types import SimpleNamespace
+
+    from junqi_b200.collector import RolloutCollector
+    mask, want = torch.ones(2, 4, dtype=torch.uint8), [torch.full((2,), float(k)) for k in (1, 2, 3)]
+    col = RolloutCollector.__new__(RolloutCollector)
+    col.env = SimpleNamespace(observe=lambda seats, seats_per_env: (None, None), mask=mask, n=2, device="cpu",
+                              batch={"terminated": torch.tensor([0, 1])})
+    col.policy = lambda sp, gl, m: kind(want)
+    col.last_values = torch.zeros(2)
+    for got, w in zip(col._act(), want):
+        assert torch.equal(got, w)
+    col._final()
+    assert col.last_values.tolist() == [3.0, 0.0]
