@@ -87,8 +87,11 @@ void no_tangent(const char *what, std::initializer_list<const Tensor *> inputs) 
         REQUIRE(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
 }
 
+// `t` as its memory has it: the imaginary part of a conjugate is negated only when torch reads it.
+Tensor read(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // `t` with neighbouring places next to each other on its last axis.
-Tensor last(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor last(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? read(t) : t.contiguous(); }
 // (rows, n) view (a copy only where the leading axes have no common stride).
 Tensor rows_of(const Tensor &t) { return last(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
 // The same inside a node's forward pass, where views have no history: with it, so that `once` finds the way back to `t`.
@@ -109,7 +112,7 @@ Tensor ints(const char *what, const Tensor &t, at::IntArrayRef shape, int64_t lo
 Tensor uniform(const char *what, const Tensor &u, at::IntArrayRef shape) {
     REQUIRE(u.scalar_type() == at::kFloat && u.sizes() == shape, what, " must be float32 ", shape_of(shape), ", got ",
             u.scalar_type(), " ", shape_of(u.sizes()));
-    return u.contiguous();
+    return read(u).contiguous();
 }
 
 // The mask, expanded to `shape`; undefined without one.
@@ -216,7 +219,7 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
     }
     REQUIRE(!weight || !bias || weight->scalar_type() == bias->scalar_type(), "layer_norm: weight and bias must have one type");
     no_tangent("layer_norm", {&x, weight ? &*weight : &x, bias ? &*bias : &x});
-    const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+    const Tensor w = weight ? read(*weight).contiguous() : Tensor(), b = bias ? read(*bias).contiguous() : Tensor();
     same_device("layer_norm", x, {&w, &b});
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
         return LayerNorm::apply(x, weight ? MaybeTensor(w) : MaybeTensor(), bias ? MaybeTensor(b) : MaybeTensor(), eps);
@@ -265,7 +268,7 @@ struct ActionLogProb : torch::autograd::Function<ActionLogProb> {
             dx = at::empty(shape, x2.options());
             if (x2.size(0) > 0) {
                 On on(x2);
-                const Tensor u = grads[0].defined() ? grads[0].reshape({-1}) : Tensor(), v = grads[1].defined() ? grads[1].reshape({-1}) : Tensor();
+                const Tensor u = grads[0].defined() ? read(grads[0]).reshape({-1}) : Tensor(), v = grads[1].defined() ? read(grads[1]).reshape({-1}) : Tensor();
                 check(api.log_prob_backward(ptr(x2), x2.stride(0), dtype_of("logits", x2), ptr<uint32_t>(bits),
                                             ptr<float>(stats), ptr<float>(u), u.defined() ? u.stride(0) : 0, ptr<float>(v),
                                             v.defined() ? v.stride(0) : 0, x2.size(0), (int32_t)x2.size(1), ptr(dx), on.stream),

@@ -191,3 +191,57 @@ def test_log_probabilities_of_kept_drafts_of_any_number_of_games(games, n, dtype
         xd = x[k:k + 100, 0].double()
         want = xd.gather(1, a[k:k + 100])[:, 0] - xd.logsumexp(1)
         within(v.log_probs[k:k + 100, 0], want, 1.01 * (92 + 6 * max(n / 256, 1) + want.abs()) * U, "log_probs")
+
+
+# -- tensors that are negated when they are read ------------------------------------------------------
+
+def lazily_negated(t):
+    """t, as the imaginary part of a conjugate: memory holds -t, and a bit says so."""
+    v = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert v.is_neg() and torch.equal(v.resolve_neg(), t)
+    return v
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_lazily_negated_inputs(n):
+    x, w, b, dy = (torch.randn(s, generator=gen(k), device="cuda") for k, s in enumerate([(5, n), (n,), (n,), (5, n)]))
+    lazy = lazily_negated
+
+    def norm(x, w, b, dy):
+        x, w, b = (v.detach().requires_grad_(True) for v in (x, w, b))
+        y = P.layer_norm(x, w, b)
+        with torch.no_grad():
+            assert torch.equal(y, P.layer_norm(x, w, b))
+        return y, *torch.autograd.grad(y, (x, w, b), dy)
+
+    for got, want in zip(norm(lazy(x), lazy(w), lazy(b), lazy(dy)), norm(x, w, b, dy)):
+        assert torch.equal(got, want)
+    a = torch.randint(0, n, (5,), generator=gen(7), device="cuda")
+    u, r = (torch.rand(5, generator=gen(s), device="cuda") for s in (8, 9))
+
+    def logp(x, u, r):
+        x = x.detach().requires_grad_(True)
+        out = P.action_log_prob(x, None, a)
+        return *out, *torch.autograd.grad(out, x, (u, r)), *P.action_log_prob(x.detach(), None, a)
+
+    for k in (slice(0, 5), slice(0, 1)):
+        for got, want in zip(P.sample_actions(lazy(x[k]), None, lazy(r[k])), P.sample_actions(x[k], None, r[k])):
+            assert torch.equal(got, want)
+        x2, y2 = x[k, None].expand(-1, 2, -1).contiguous(), dy[k, None].contiguous()
+        for got, want in zip(P.verify_drafts(lazy(x2), a[k, None], lazy(u[k, None]), lazy(r[k]), draft_logits=lazy(y2)),
+                             P.verify_drafts(x2, a[k, None], u[k, None], r[k], draft_logits=y2)):
+            assert torch.equal(got, want)
+    for got, want in zip(logp(lazy(x), lazy(u), lazy(r)), logp(x, u, r)):
+        assert torch.equal(got, want)
+
+
+def test_gradients_through_a_conjugate():
+    """What torch hands to the backward pass of a value that went into a complex number."""
+    x = torch.randn(6, 20, generator=gen(1), device="cuda", requires_grad=True)
+    a = torch.randint(0, 20, (6,), generator=gen(2), device="cuda")
+    c = torch.randn(6, generator=gen(3), device="cuda")
+    for op in (lambda: P.action_log_prob(x, None, a)[0], lambda: P.action_log_prob(x, None, a)[1], lambda: P.layer_norm(x)[:, 3]):
+        v = op()
+        (got,) = torch.autograd.grad((torch.complex(torch.zeros_like(v), v).conj().imag * c).sum(), x)
+        (want,) = torch.autograd.grad((op() * -c).sum(), x)
+        assert torch.equal(got, want)
