@@ -374,17 +374,18 @@ enum { JQ_F32 = 0, JQ_F16 = 1, JQ_BF16 = 2 };
 
 /* Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight +
  * bias (either may be NULL: 1 and 0).  x, y are `dtype`, weight and bias
- * `wdtype` (JQ_F32 or `dtype`); statistics are 32-bit.  d_stats (rows x 3
- * floats: mean, what its rounding left, 1 / sqrt(var + eps)) is what the
- * backward pass reads, NULL when there will be none.  1 <= rows < 2^31,
- * 1 <= dim <= 2^30. */
+ * `wdtype` (JQ_F32 or `dtype`); statistics are 32-bit, so a row's sum has to
+ * be a number of 32 bits.  d_stats (rows x 3 floats: mean, what its rounding
+ * left, 1 / sqrt(var + eps)) is what the backward pass reads, NULL when there
+ * will be none.  1 <= rows < 2^31, 1 <= dim <= 2^30. */
 int jq_layer_norm(const void *d_x, int64_t x_stride, const void *d_weight, const void *d_bias, int64_t rows,
                   int32_t dim, int32_t dtype, int32_t wdtype, float eps, void *d_y, float *d_stats, void *stream);
 
 /* Gradients of jq_layer_norm from dy (`dtype`): d_dx (`dtype`), d_dweight and
- * d_dbias (`wdtype`, summed over the rows in a fixed order); each may be
- * NULL.  d_scratch: jq_layer_norm_scratch_floats(rows, dim) floats, needed
- * for d_dweight and d_dbias, used by one call at a time. */
+ * d_dbias (`wdtype`, summed over the rows in a fixed order: a CTA's rows in 32
+ * bits, the CTAs' sums in 64); each may be NULL.  d_scratch:
+ * jq_layer_norm_scratch_floats(rows, dim) floats, needed for d_dweight and
+ * d_dbias, used by one call at a time. */
 int64_t jq_layer_norm_scratch_floats(int64_t rows, int32_t dim);
 int jq_layer_norm_backward(const void *d_x, int64_t x_stride, const void *d_weight, const void *d_dy,
                            int64_t dy_stride, const float *d_stats, int64_t rows, int32_t dim, int32_t dtype,

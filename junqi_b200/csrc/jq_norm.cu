@@ -29,10 +29,14 @@
 // per row go to the backward pass.
 //
 // Measured (B200, 264,192 rows of 256 bfloat16): forward 47 us (5.8 TB/s, 0.89
-// of a plain copy's rate), backward 70 us (5.8 TB/s) and 3 us for the second
-// kernel.  Rows of a CTA wait for its barriers: 6,000 rows of 4,096 float16
-// take 29 and 43 us (3.4 TB/s, 62 and 43 % of the issue slots), 8,191 of 1,111
-// float32, whose rows start anywhere, 20 and 25 us (3.7 and 4.3 TB/s).
+// of a plain copy's rate), backward 70 us (5.8 TB/s) and 6.5 us for the second
+// kernel after a flush; pass after pass 73 us without the weights' gradients and
+// 79 with them.  Rows of a CTA wait for its barriers: 6,000 rows of 4,096
+// float16 take 28 and 43 us (3.5 TB/s, 63 and 43 % of the issue slots), 8,191
+// of 1,111 float32, whose rows start anywhere, 19 and 25 us (3.8 and 4.3 TB/s).
+// Rows of one or two places, whose threads hold mostly nothing, spill up to 60
+// bytes: 3,000,017 rows of 1 float32 take 70 and 70 us, of 16 bfloat16 (half as
+// many) 30 and 42.
 #include <atomic>
 
 #include "jq_ops.cuh"
@@ -529,7 +533,9 @@ __global__ void __launch_bounds__(512) norm_dw_kernel(const float *part, int par
 
 // Rows longer than the registers hold: a CTA per row that reads it again for
 // each sum (from L2, where one row stays), and for the weights' gradients a
-// thread per column over a share of the rows.
+// thread per column over a share of the rows.  One element a load: 4,096 rows
+// of 8,200 bfloat16 take 80 us forward and 272 both ways, of 16,384 145 and 591
+// (8,192 places, in registers: 42 and 101).
 template <typename T>
 __global__ void __launch_bounds__(512, 4) norm_fwd_long_kernel(const NormArgs a) {
     __shared__ float sm1[2][NORM_WARPS][1], sm2[2][NORM_WARPS][2];

@@ -324,9 +324,10 @@ __global__ void __launch_bounds__(32 * LOGP_WARPS, 9) logp_masked_kernel(const L
         for (int w = lane; w < a.words; w += 32) a.bits[row * a.words + w] = legal.word(w, a.n);
 }
 
-// Without: a CTA per row, 16 bytes a load, the ends one by one.  Close to its
-// bound: 30 us for 2,048 rows of 30,001 float16 (4.1 TB/s, two thirds of the
-// issue slots; the exponentials alone need 14 us of the special function units).
+// Without: a CTA per row, 16 bytes a load, the ends one by one.  31 us for 2,048
+// rows of 30,001 float16 (4.0 TB/s, 0.61 of a plain copy's rate; two thirds of
+// the issue slots, and the exponentials alone need 14 us of the special function
+// units: nothing of these is full).
 template <typename T>
 __global__ void __launch_bounds__(LOGP_THREADS, 6) logp_dense_kernel(const LogpArgs a) {
     constexpr int VEC = 16 / sizeof(T);
@@ -502,11 +503,13 @@ __global__ void __launch_bounds__(LOGP_THREADS) logp_bwd_kernel(const LogpArgs a
 // That is with a mask, where a place is one warp's: it packs the mask, lists
 // the legal actions in order, and does the rest on the list without a barrier;
 // what bounds it is the mask's bytes (with many games) or the chain of some
-// thousand cycles (with few).  Without a mask the bound is the exponentials in
-// 64 bits (verify_dense_kernel).  Measured: 4,096 samples of 16,641 float32 with
+// thousand cycles (with few).  Measured: 4,096 samples of 16,641 float32 with
 // up to 80 legal actions 20 us (69 MB, 3.4 TB/s), 8 games of 4 drafts 8.9 us,
 // 1,024 of up to 8 drafts 43 us; place by place and a CTA per game these took
-// 89, 33 and 125.  301 games of 5 drafts without a mask 67 us.
+// 89, 33 and 125.  1,024 games of 8 bare drafts 32 us.  Without a mask
+// (verify_dense_kernel) 301 games of 5 drafts take 66 us, of which the 64-bit
+// operations are about 15 at the chip's rate, and 64-bit exchanges, spills and
+// the 32-bit pass over places behind a rejection the rest.
 
 constexpr int VERIFY_WARPS = 36;  // of an SM, for the launch
 constexpr double RESIDUAL_MIN = 1.0 / (double)(1ull << 40);  // less left after a rejection counts as none
@@ -520,9 +523,8 @@ struct VerifyArgs {
 // e^d for d <= 0 in 64 bits: d = k ln 2 / 16 + r, e^d = 2^(k / 16) e^r, from a
 // table of 16 and five terms of the series (Tang's table-driven exponential,
 // ACM TOMS 1989); |r| <= 0.0217, so the sixth is below 1.5e-13.  Below -700: 0.
-// Ten operations, where the library's function has about three times that:
-// without a mask they are the kernel's bound.  16 entries, because they lie in
-// banks of their own.
+// Good to 1.7e-13 relatively.  Ten operations, where the library's function has
+// about three times that.  16 entries, because they lie in banks of their own.
 constexpr int EXP_STEPS = 16;
 __device__ __forceinline__ double exp_table(int i) { return exp2((double)i / EXP_STEPS); }
 // 16 / ln 2, -ln 2 / 16, 1 / 5!, 1 / 4!, 1 / 3!: as constants in memory they are operands; written into the code,
@@ -1130,7 +1132,8 @@ static int verify_launch(const jq_drafts &d, cudaStream_t s) {
     if (!d.mask) {
         int sms, rc = device_sms(sms);
         if (rc) return rc;
-        // enough CTAs to fill the SMs once (4 each), of a thousand places or more: each place costs every warp an exchange
+        // CTAs of a thousand places or more until the SMs are full (4 each; up to twice that, and no step shows where it is
+        // passed: 296 games 65.7 us, 297 66.1, 301 65.7): each place costs every warp an exchange
         int ctas = 1;
         while (ctas < DENSE_CTAS && (int64_t)d.games * ctas < 4 * (int64_t)sms && d.actions > 1024 * ctas) ctas *= 2;
         if ((int64_t)d.games * ctas > INT32_MAX) return fail(JQ_ERR_CAPACITY, "drafts: too many games for one call");

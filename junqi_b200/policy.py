@@ -88,7 +88,10 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, accept_u: torch.Te
     kept drafts without a mask come from 32-bit sums: off by (92 + 6 n / 256) 2^-24
     at most, measured below 2^-17 up to 262,144 actions).  A place without legal
     actions gives -1, one with NaN or +inf at a legal place -1 and a NaN
-    log-probability.  Not differentiable: see :func:`action_log_prob`."""
+    log-probability.  Not differentiable: see :func:`action_log_prob`.
+
+    An environment does not go back to the ply of a rejection: draft on a batch of
+    which another one holds the positions to play on from."""
     return Verified(*N.policy().verify_drafts(logits, drafts, accept_u, sample_u, draft_logits, mask, lengths))
 
 
