@@ -136,7 +136,7 @@ def build(force: bool = False, trace: bool = False) -> Path:
     if other:
         POLICY_PATH.unlink()  # file times do not show it
     if force or stale or other:
-        subprocess.run(["make", "-s", "-C", str(CSRC), f"PYTHON={sys.executable}"] + (["trace"] if trace else []),
+        subprocess.run(["make", "-s", "-j4", "-C", str(CSRC), f"PYTHON={sys.executable}"] + (["trace"] if trace else []),
                        check=True)
     return path
 
